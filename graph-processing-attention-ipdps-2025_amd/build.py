@@ -35,9 +35,10 @@ HIP_FLAGS = [
 
 ELEM_TYPES = {"f32": "float", "f16": "spfa::f16", "bf16": "spfa::bf16"}
 MASK_KINDS = {"csr": 0, "stride": 1, "global": 2}
+CACHE_CODES = {"none": 0, "int8": 1, "e4m3": 2}
 
 MODULES = ["spfa_csr", "spfa_coo", "spfa_local", "spfa_local_1d_dilated", "spfa_local_2d_dilated",
-           "spfa_global_no_local", "spfa_bigbird"]
+           "spfa_global_no_local", "spfa_bigbird", "spfa_rope", "spfa_cache", "spfa_tree"]
 
 
 def _run(cmd):
@@ -60,8 +61,14 @@ def lib_jobs():
             jobs.append((obj, [HIPCC, *HIP_FLAGS, "-DSPFA_INST_MASK=%d" % mid,
                                "-DSPFA_INST_T=%s" % tcpp, "-c",
                                os.path.join(CSRC, "spfa_grad_inst.hip"), "-o", obj]))
+    for tname in ("f16", "bf16"):
+        for cname, cid in CACHE_CODES.items():
+            obj = os.path.join(OBJ, "tree_%s_%s.o" % (tname, cname))
+            jobs.append((obj, [HIPCC, *HIP_FLAGS, "-DSPFA_TREE_T=%s" % ELEM_TYPES[tname],
+                               "-DSPFA_TREE_CODE=%d" % cid, "-c",
+                               os.path.join(CSRC, "spfa_tree_inst.hip"), "-o", obj]))
     for src in sorted(os.listdir(CSRC)):
-        if src.endswith(".hip") and src not in ("spfa_inst.hip", "spfa_grad_inst.hip"):
+        if src.endswith(".hip") and src not in ("spfa_inst.hip", "spfa_grad_inst.hip", "spfa_tree_inst.hip"):
             obj = os.path.join(OBJ, src[:-4] + ".o")
             jobs.append((obj, [HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]))
     return jobs

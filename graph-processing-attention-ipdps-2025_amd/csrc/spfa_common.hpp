@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace spfa {
 
 constexpr int kWave = 64;
@@ -366,6 +368,24 @@ __device__ __forceinline__ int listed_token(int g, int64_t n) {
 
 __device__ __forceinline__ int lane_id() {
   return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+}
+
+// Raises a kernel's dynamic-LDS limit to `bytes`, once per device: `raised` is the caller's table
+// of kLdsLimitDevices flags for that kernel (atomic: callers may be on several host threads; two
+// that meet here both set the attribute, which is idempotent).  A device beyond the table gets
+// the attribute set on every call.  False when the runtime refuses.
+constexpr int kLdsLimitDevices = 64;
+inline bool raise_lds_limit(const void* kernel, int bytes, std::atomic<bool>* raised) {
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess) return false;
+  const bool tabled = dev >= 0 && dev < kLdsLimitDevices;
+  if (tabled && raised[dev].load(std::memory_order_acquire)) return true;
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) {
+    (void)hipGetLastError();
+    return false;
+  }
+  if (tabled) raised[dev].store(true, std::memory_order_release);
+  return true;
 }
 
 }  // namespace spfa

@@ -105,3 +105,48 @@ def attention(q, k, v, parts, return_state=False):
         _module(p[0])
     out, m, l = _MaskedAttention.apply(q, k, v, parts)
     return (out, m, l) if return_state else out
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, w_q, w_k, positions, inv_freq, eps, interleaved, heads_first):
+        q, k = (x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous() for x in (q, k))
+        q_out, k_out = (_like_heads(x, heads_first) for x in (q, k))
+        importlib.import_module("spfa_rope").forward(q, k, w_q, w_k, positions, inv_freq, q_out, k_out, eps, interleaved)
+        ctx.save_for_backward(q, k, w_q, w_k, positions, inv_freq)
+        ctx.how = (eps, interleaved, heads_first)
+        if heads_first:
+            return q_out.transpose(-3, -2), k_out.transpose(-3, -2)
+        return q_out, k_out
+
+    @staticmethod
+    def backward(ctx, d_q_out, d_k_out):
+        q, k, w_q, w_k, positions, inv_freq = ctx.saved_tensors
+        eps, interleaved, heads_first = ctx.how
+        d_q, d_k = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        d_w = [None if w is None or not need else torch.empty(w.shape, dtype=torch.float32, device=w.device)
+               for w, need in zip((w_q, w_k), ctx.needs_input_grad[2:4])]
+        outs = [d.transpose(-3, -2) if heads_first else d for d in (d_q_out, d_k_out)]
+        outs = [d if d.stride(-1) == 1 or d.shape[-1] <= 1 else d.contiguous() for d in outs]
+        importlib.import_module("spfa_rope").backward(q, k, w_q, w_k, positions, inv_freq, *outs, d_q, d_k, *d_w, eps, interleaved)
+        d_w = [None if d is None else d.to(w.dtype) for d, w in zip(d_w, (w_q, w_k))]
+        return d_q, d_k, *d_w, None, None, None, None, None
+
+
+def _like_heads(x, heads_first):
+    """An uninitialised tensor of x's shape, its heads outside its tokens in memory if heads_first."""
+    if heads_first:
+        shape = (*x.shape[:-3], x.shape[-2], x.shape[-3], x.shape[-1])
+        return torch.empty(shape, dtype=x.dtype, device=x.device).transpose(-3, -2)
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def qk_norm_rope(q, k, w_q, w_k, positions, inv_freq, eps=1e-6, interleaved=False, heads_first=True):
+    """Head norms of queries and keys with the position rotation (spfa_rope), differentiable in q, k,
+    w_q and w_k.
+
+    q, k: [tokens, heads, d] or [batch, tokens, heads, d], any strides outside the last dimension (the
+    slices of a fused projection are fine); w_q, w_k: [d] or None; positions: [tokens] or
+    [batch, tokens] integers; inv_freq: float32 [pairs].  Returns (q, k) as attention() takes them,
+    [..., heads, tokens, d], or in the order of the inputs with heads_first=False."""
+    return _QkNormRope.apply(q, k, w_q, w_k, positions, inv_freq, eps, interleaved, heads_first)

@@ -70,3 +70,35 @@ def stack_csr_masks(masks, n_cols):
     if len(masks) * n_cols >= 1 << 32:
         raise ValueError("stacked column indices do not fit 32 bits")
     return torch.cat(offs).to(torch.uint64).contiguous(), torch.cat(cols).to(torch.uint32).contiguous()
+
+
+def tree_mask(parents, q_offsets=None, device=None):
+    """The ancestor bits spfa_tree.forward() takes as tree_mask, from parent pointers.
+
+    parents: for every drafted token the index of its parent within its own sequence's tree, -1 for a
+    node that hangs on the last cached token; a parent comes before its children.  q_offsets: where
+    the sequences begin in `parents` (as in spfa_tree.forward; None: one sequence).  Row i has bit j
+    set when node j is node i or one of its ancestors.  Returns int64 [rows, words] on `device` (that
+    of `parents` when it is a tensor)."""
+    if torch.is_tensor(parents):
+        device = parents.device if device is None else device
+        parents = parents.tolist()
+    if q_offsets is None:
+        q_offsets = [0, len(parents)]
+    elif torch.is_tensor(q_offsets):
+        q_offsets = q_offsets.tolist()
+    if not q_offsets or q_offsets[0] < 0 or q_offsets[-1] > len(parents) or any(a > b for a, b in zip(q_offsets, q_offsets[1:])):
+        raise ValueError("q_offsets must ascend within the rows of parents")
+    longest = max([b - a for a, b in zip(q_offsets, q_offsets[1:])], default=0)
+    words = max(1, -(-longest // 64))
+    bits = [0] * len(parents)
+    for a, b in zip(q_offsets, q_offsets[1:]):
+        for i in range(b - a):
+            p = parents[a + i]
+            if not -1 <= p < i:
+                raise ValueError("the parent of a node must be -1 or a node before it")
+            bits[a + i] = (1 << i) | (bits[a + p] if p >= 0 else 0)
+    low = (1 << 64) - 1
+    rows = [[(x >> (64 * w)) & low for w in range(words)] for x in bits]
+    rows = [[x - (1 << 64) if x >> 63 else x for x in r] for r in rows]
+    return torch.tensor(rows, dtype=torch.int64, device=device).reshape(len(parents), words)

@@ -341,6 +341,130 @@ int spfa_window_global_csr_backward(const spfa_problem_t* p, const spfa_grads_t*
                                     const uint32_t* t_row_off, const uint32_t* t_col_ind, void* workspace,
                                     size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Head norms with the position rotation.  The reference starts from finished Q and K
+ * (sp_flatt_csr.cpp:28-39); the models that call it norm and rotate them first.  One pass over
+ * the queries and keys of a layer, for each token t and head h:
+ *     n = x / sqrt(mean(x^2) + eps),  y = n * w,  out = y with its first `rot` elements rotated:
+ *     pair i (i < rot / 2) turned by the angle position[t] * inv_freq[i]
+ * A pair is (i, i + rot / 2), with interleaved != 0 (2 i, 2 i + 1).  Sums are fp32, angles are
+ * reduced in fp64 (any position a 64-bit integer holds up to 2^53), outputs are rounded once.
+ *
+ * spfa_heads_t: [batch, tokens, heads, d] with unit stride along d and any strides (in elements)
+ * along the others; an output may not overlap itself or the other tensors, except that it may be
+ * the very tensor it is computed from (q_out == q with the same strides). */
+typedef struct spfa_heads {
+  void* data;
+  int64_t stride_batch, stride_token, stride_head;
+} spfa_heads_t;
+
+typedef struct spfa_rope {
+  int64_t batch, tokens;
+  int64_t heads_q, heads_k;       /* either may be 0 */
+  int64_t d;                      /* 1 <= d <= 1024 */
+  int64_t rot;                    /* rotated elements of a head: even, 0 <= rot <= d */
+  int32_t dtype;                  /* SPFA_DTYPE_F32, _F16 or _BF16: q, k and outputs */
+  int32_t w_dtype;                /* the same, or SPFA_DTYPE_F32: w_q, w_k */
+  int32_t position_bytes;         /* 4 or 8: signed integers */
+  int32_t interleaved;
+  float eps;
+  spfa_heads_t q, k;
+  const void* w_q;                /* [d], NULL: ones */
+  const void* w_k;
+  const void* positions;          /* element [b * position_stride + t] is token t's of batch b */
+  int64_t position_stride;        /* 0: one row of positions for every batch entry */
+  const float* inv_freq;          /* [rot / 2] */
+} spfa_rope_t;
+
+int spfa_qk_norm_rope_forward(const spfa_rope_t* p, const spfa_heads_t* q_out, const spfa_heads_t* k_out,
+                              void* stream);
+/* Gradients: d_q_out, d_k_out are those of the outputs; d_q, d_k (element type of the problem) and
+ * d_w_q, d_w_k (fp32 [d], either may be NULL) are WRITTEN, not added to.  The weights' sums over
+ * tokens and heads run in an order that depends on the sizes alone. */
+size_t spfa_qk_norm_rope_backward_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads_q,
+                                                  int64_t heads_k, int64_t d);
+int spfa_qk_norm_rope_backward(const spfa_rope_t* p, const spfa_heads_t* d_q_out, const spfa_heads_t* d_k_out,
+                               const spfa_heads_t* d_q, const spfa_heads_t* d_k, float* d_w_q, float* d_w_k,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * A paged cache of keys and values, plain or in 8 bits.  Pages hold page_size tokens of `heads`
+ * rows of d elements (unit stride along d, any strides along page, place in the page and head, in
+ * elements); slot s is place s % page_size of page s / page_size.
+ *   SPFA_CODE_NONE  rows of the element type of k and v, no scales
+ *   SPFA_CODE_INT8  code = round(x * 127 / amax), ties to even, scale = amax / 127
+ *   SPFA_CODE_E4M3  code = x * 448 / amax rounded to 4 significant bits (OCP e4m3), ties to even,
+ *                   scale = amax / 448
+ * with amax the largest absolute value of the row (one row per token and head, K and V apart); the
+ * quotient is rounded as if it were exact.  A row of zeros has scale 0; a row that holds an
+ * infinity or a NaN reads back as NaN.  Values read back are code * scale (fp32), rounded once.
+ *
+ * Slots outside [0, pages * page_size) are skipped: nothing is written, or the output row stays as
+ * it was.  The slots of one write must differ from each other (skipped ones apart): of a slot
+ * listed twice the rows are unspecified, though never written out of place. */
+enum { SPFA_CODE_NONE = 0, SPFA_CODE_INT8 = 1, SPFA_CODE_E4M3 = 2 };
+
+typedef struct spfa_cache {
+  void* k;                        /* [pages, page_size, heads, d] by the strides below */
+  void* v;
+  float* k_scale;                 /* [pages, page_size, heads]; NULL for SPFA_CODE_NONE */
+  float* v_scale;
+  int64_t k_stride_page, k_stride_slot, k_stride_head;
+  int64_t v_stride_page, v_stride_slot, v_stride_head;
+  int64_t ks_stride_page, ks_stride_slot, ks_stride_head;
+  int64_t vs_stride_page, vs_stride_slot, vs_stride_head;
+  int64_t pages, page_size, heads, d;   /* 1 <= d <= 1024 */
+  int32_t code;                   /* SPFA_CODE_* */
+  int32_t dtype;                  /* SPFA_DTYPE_F32, _F16 or _BF16: of k and v outside the cache */
+} spfa_cache_t;
+
+/* k, v: [tokens, heads, d] (stride_batch unused); slots: `tokens` signed integers of slot_bytes
+ * (4 or 8) bytes each. */
+int spfa_cache_write(const spfa_cache_t* c, const spfa_heads_t* k, const spfa_heads_t* v, int64_t tokens,
+                     const void* slots, int slot_bytes, void* stream);
+int spfa_cache_read(const spfa_cache_t* c, const void* slots, int slot_bytes, int64_t tokens,
+                    const spfa_heads_t* k_out, const spfa_heads_t* v_out, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Attention of drafted tokens over a paged cache.  Sequence s owns rows q_offsets[s] ..
+ * q_offsets[s+1] of q: the nodes of its tree.  Their keys and values are already in the cache,
+ * node i at position ctx_lens[s] + i of the sequence; position x is place x % page_size of page
+ * page_table[s][x / page_size].  Node i attends
+ *   - every position before ctx_lens[s], and
+ *   - node j of its own tree when bit j % 64 of tree_mask[row of i][j / 64] is set; without a mask
+ *     (NULL) every j <= i: a chain, i.e. plain decoding (one node) or a chunk of a prompt.
+ * heads_q must be a multiple of the cache's heads; head h reads cache head h / (heads_q / heads).
+ * out = softmax(scale * q k^T) v.  With m and l given, (m, l, out) is in/out state with the
+ * meaning it has in the calls above (out normalised; m in units of scale * q.k), so the call chains
+ * with others on the same rows, and rows with nothing to attend keep all three.  Without them (both
+ * NULL) rows start afresh and a row with nothing to attend becomes zeros.  Rows of q outside
+ * [q_offsets[0], q_offsets[n_seqs]) are left as they were.
+ *
+ * The arrays on the device are held to the sizes given here: a position whose page entry is not in
+ * [0, pages) or lies past page_table is masked, a negative ctx_len counts as 0, offsets are cut to
+ * [0, rows], nodes past 64 * mask_words have no bits.  What masked places hold (NaN included) does
+ * not reach a row that masks them. */
+typedef struct spfa_tree {
+  const void* q;                  /* [rows, heads_q, d], unit stride along d */
+  void* out;                      /* likewise */
+  int64_t q_stride_row, q_stride_head, out_stride_row, out_stride_head;
+  float* m;                       /* [rows, heads_q] contiguous, or NULL */
+  float* l;
+  int64_t rows, heads_q, n_seqs;
+  const int32_t* q_offsets;       /* [n_seqs + 1], ascending */
+  const int32_t* ctx_lens;        /* [n_seqs] */
+  const int32_t* page_table;      /* [n_seqs, table_width], rows table_stride apart */
+  int64_t table_width, table_stride;
+  const int64_t* tree_mask;       /* [rows, mask_words] contiguous, or NULL */
+  int64_t mask_words;
+  float scale;
+} spfa_tree_t;
+
+/* The cache's dtype (SPFA_DTYPE_F16 or _BF16) is that of q and out too; d <= 256. */
+size_t spfa_tree_workspace_bytes(const spfa_cache_t* c, const spfa_tree_t* t);
+int spfa_tree_forward(const spfa_cache_t* c, const spfa_tree_t* t, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif
