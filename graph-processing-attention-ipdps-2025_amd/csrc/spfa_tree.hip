@@ -1,26 +1,40 @@
 // C entry points of the tree attention (spfa_tree.hpp): checks, choice of kernel, workspace.
 #include "spfa_tree.hpp"
 
+#include <cfloat>
+#include <cmath>
+#include <initializer_list>
+
 namespace spfa {
-template <> int tree_run<f16, SPFA_CODE_NONE>(const TreeArgs&, int, int, int, bool, hipStream_t);
-template <> int tree_run<f16, SPFA_CODE_INT8>(const TreeArgs&, int, int, int, bool, hipStream_t);
-template <> int tree_run<f16, SPFA_CODE_E4M3>(const TreeArgs&, int, int, int, bool, hipStream_t);
-template <> int tree_run<bf16, SPFA_CODE_NONE>(const TreeArgs&, int, int, int, bool, hipStream_t);
-template <> int tree_run<bf16, SPFA_CODE_INT8>(const TreeArgs&, int, int, int, bool, hipStream_t);
-template <> int tree_run<bf16, SPFA_CODE_E4M3>(const TreeArgs&, int, int, int, bool, hipStream_t);
+template <> int tree_run<f16, SPFA_CODE_NONE>(const TreeArgs&, const TreeShape&, hipStream_t);
+template <> int tree_run<f16, SPFA_CODE_INT8>(const TreeArgs&, const TreeShape&, hipStream_t);
+template <> int tree_run<f16, SPFA_CODE_E4M3>(const TreeArgs&, const TreeShape&, hipStream_t);
+template <> int tree_run<bf16, SPFA_CODE_NONE>(const TreeArgs&, const TreeShape&, hipStream_t);
+template <> int tree_run<bf16, SPFA_CODE_INT8>(const TreeArgs&, const TreeShape&, hipStream_t);
+template <> int tree_run<bf16, SPFA_CODE_E4M3>(const TreeArgs&, const TreeShape&, hipStream_t);
 
 namespace {
 
 constexpr int64_t kMaxPositions = INT32_MAX - 1024;
 
 struct TreePlan {
-  int rows_how, dp, rb, wave_rows, workers;
-  bool merge;
+  TreeShape shape;
+  int workers;
   size_t part_bytes, state_bytes, acc_bytes;
   size_t bytes() const { return part_bytes + 2 * state_bytes + acc_bytes + 256; }
 };
 
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// p / d for p < 2^31 as (p * magic >> 32) >> shift (shift < 0: d is 1).  With s the bits of d - 1 and
+// magic = ceil(2^(31 + s) / d) < 2^32, p * magic exceeds p * 2^(31 + s) / d by less than
+// p / 2^31 * 2^(31 + s) / d, too little to reach the next whole quotient.
+void tree_divider(int32_t d, uint32_t* magic, int32_t* shift) {
+  int s = 0;
+  while (((int64_t)1 << s) < d) s++;
+  *shift = s - 1;
+  *magic = s == 0 ? 0u : (uint32_t)((((uint64_t)1 << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d);
+}
 
 int tree_check(const spfa_cache_t* c, const spfa_tree_t* t) {
   if (c == nullptr || t == nullptr) return SPFA_ERR_BAD_ARG;
@@ -32,6 +46,13 @@ int tree_check(const spfa_cache_t* c, const spfa_tree_t* t) {
     return SPFA_ERR_BAD_ARG;
   if (t->rows < 0 || t->rows > INT32_MAX || t->n_seqs < 0 || t->n_seqs > (1 << 24)) return SPFA_ERR_BAD_ARG;
   if (t->table_width < 0 || t->mask_words < 0) return SPFA_ERR_BAD_ARG;
+  // (a row and a query head of its group make one number of 31 bits)
+  if (t->rows > (INT32_MAX - 1024) / (t->heads_q / c->heads)) return SPFA_ERR_UNSUPPORTED;
+  // (the kernels multiply page numbers and places by 32-bit strides)
+  const int64_t limit = INT32_MAX;
+  for (int64_t s : {c->k_stride_page, c->k_stride_slot, c->v_stride_page, c->v_stride_slot, c->ks_stride_page, c->ks_stride_slot,
+                    c->vs_stride_page, c->vs_stride_slot})
+    if (s < 0 || s > limit) return SPFA_ERR_UNSUPPORTED;
   if ((t->m == nullptr) != (t->l == nullptr)) return SPFA_ERR_BAD_ARG;
   return SPFA_OK;
 }
@@ -46,27 +67,39 @@ TreePlan tree_plan(const spfa_cache_t* c, const spfa_tree_t* t) {
                        ((uintptr_t)t->q & 15) == 0 && whole(c->k_stride_page, es) && whole(c->k_stride_slot, es) &&
                        whole(c->k_stride_head, es) && whole(c->v_stride_page, es) && whole(c->v_stride_slot, es) &&
                        whole(c->v_stride_head, es) && whole(t->q_stride_row, 2) && whole(t->q_stride_head, 2);
-  p.dp = c->d <= 64 ? 64 : c->d <= 128 ? 128 : 256;
-  p.rows_how = !aligned ? kTreeAny : c->d == p.dp ? kTreeWhole : kTreePadded;
-  // rows of an average sequence and head: as many wavefronts side by side as they fill, the others
-  // share the keys
+  TreeShape& s = p.shape;
+  s.dp = c->d <= 64 ? 64 : c->d <= 128 ? 128 : 256;
+  s.rows_how = !aligned ? kTreeAny : c->d == s.dp ? kTreeWhole : kTreePadded;
+  // The rows and keys of an average sequence and head (lengths are not known here: no more keys than the
+  // table and the cache have places).
   const int64_t group = t->heads_q / c->heads;
   const int64_t rows = t->n_seqs > 0 ? (t->rows * group + t->n_seqs - 1) / t->n_seqs : 0;
-  p.rb = rows > 32 && p.dp <= 128 && p.rows_how == kTreeWhole ? 2 : 1;
-  p.wave_rows = rows <= 32 * p.rb ? 1 : rows <= 64 * p.rb ? 2 : 4;
-  const int64_t M = 32 * p.rb * p.wave_rows;
-  // two workgroups per CU where registers and LDS hold two; no more than there can be units of work
-  const int64_t most = p.dp * p.rb <= 128 ? 512 : 256;
   const int64_t len = t->table_width < kMaxPositions / c->page_size ? t->table_width * c->page_size : kMaxPositions;
   const int64_t blocks = len <= kTreeBlock ? 1 : (len + kTreeBlock - 1) / kTreeBlock;
+  double keys = (double)len * (double)t->n_seqs;
+  if (keys > (double)c->pages * (double)c->page_size) keys = (double)c->pages * (double)c->page_size;
+  // The wide kernel takes a key's way through LDS once for 128 rows, but has to fill, store and join 128:
+  // it gains once they are more than two of the narrow kernel's tiles and its workgroups have many blocks.
+  // Us, narrow against wide, 8 sequences and 4 heads: 64 bf16/f16 elements, 96 rows of 2900 keys 28 / 35, of
+  // 20000 84 / 66, 512 of 8000 110 / 86; 128 bf16 elements, 128 rows of 20000 192 / 183, 512 of 8000
+  // 232 / 216, of 2900 97 / 106; 128 int8 elements, 128 rows of 20000 127 / 127, 192 179 / 203, 512 of 40000
+  // 770 / 651; 256 elements, 128 rows of 20000 bf16 495 / 400, e4m3 313 / 344, 512 of 8000 466 / 452.
+  const double per_group = (double)c->heads * (double)((rows + 127) / 128) * keys / kTreeBlock / (256 * wide_groups(s.dp));
+  const bool many = rows > (c->code == SPFA_CODE_NONE || s.dp == 64 ? 64 : 192);
+  s.wide = s.rows_how != kTreeAny && many && per_group >= (s.dp == 64 ? 4.0 : 16.0);
+  s.nr = s.rows_how != kTreeAny && rows > 16 && s.dp < 256 ? 2 : 1;
+  const int64_t M = s.rows();
+  // as many workgroups as are to run at a time, no more than there can be units of work
+  const int64_t most = 256 * (s.wide ? wide_groups(s.dp) : narrow_groups(c->code, s.dp));
   const int64_t tiles = t->rows * group / M + (t->n_seqs < t->rows ? t->n_seqs : t->rows);
   const double units = (double)tiles * (double)c->heads * (double)blocks;
   p.workers = units < (double)most ? (int)units : (int)most;
   if (p.workers < 1) p.workers = 1;
-  p.merge = blocks > 1;
+  // (a table of one block cuts no item; the merge has a workgroup per part and row, up to 32)
+  s.merge_rows = blocks <= 1 ? 0 : (int)(rows < 1 ? 1 : rows < 32 ? rows : 32);
   p.part_bytes = round256((size_t)p.workers * sizeof(TreePart));
-  p.state_bytes = p.merge ? round256((size_t)2 * p.workers * M * sizeof(float)) : 0;
-  p.acc_bytes = p.merge ? round256((size_t)2 * p.workers * M * p.dp * sizeof(float)) : 0;
+  p.state_bytes = s.merge_rows ? round256((size_t)2 * p.workers * M * sizeof(float)) : 0;
+  p.acc_bytes = s.merge_rows ? round256((size_t)2 * p.workers * M * s.dp * sizeof(float)) : 0;
   return p;
 }
 
@@ -106,17 +139,17 @@ extern "C" int spfa_tree_forward(const spfa_cache_t* c, const spfa_tree_t* t, vo
   a.v = (const char*)c->v;
   a.ks = c->k_scale;
   a.vs = c->v_scale;
-  a.k_page = c->k_stride_page;
-  a.k_slot = c->k_stride_slot;
+  a.k_page = (uint32_t)c->k_stride_page;
+  a.k_slot = (uint32_t)c->k_stride_slot;
   a.k_head = c->k_stride_head;
-  a.v_page = c->v_stride_page;
-  a.v_slot = c->v_stride_slot;
+  a.v_page = (uint32_t)c->v_stride_page;
+  a.v_slot = (uint32_t)c->v_stride_slot;
   a.v_head = c->v_stride_head;
-  a.ks_page = c->ks_stride_page;
-  a.ks_slot = c->ks_stride_slot;
+  a.ks_page = (uint32_t)c->ks_stride_page;
+  a.ks_slot = (uint32_t)c->ks_stride_slot;
   a.ks_head = c->ks_stride_head;
-  a.vs_page = c->vs_stride_page;
-  a.vs_slot = c->vs_stride_slot;
+  a.vs_page = (uint32_t)c->vs_stride_page;
+  a.vs_slot = (uint32_t)c->vs_stride_slot;
   a.vs_head = c->vs_stride_head;
   a.q_offsets = t->q_offsets;
   a.ctx_lens = t->ctx_lens;
@@ -133,9 +166,15 @@ extern "C" int spfa_tree_forward(const spfa_cache_t* c, const spfa_tree_t* t, vo
   a.d = (int32_t)c->d;
   a.page_size = (int32_t)c->page_size;
   a.max_len = !keys ? 0 : t->table_width < kMaxPositions / c->page_size ? (int32_t)(t->table_width * c->page_size) : (int32_t)kMaxPositions;
-  a.scale_log2 = t->scale * 1.4426950408889634f;
+  tree_divider(a.page_size, &a.page_magic, &a.page_shift);
+  tree_divider(a.group, &a.group_magic, &a.group_shift);
+  tree_divider(p.shape.rows(), &a.tile_magic, &a.tile_shift);
+  // the kernels look for the largest score before they scale it: a negative scale becomes the queries'
+  // sign, and zero the smallest number there is (masked scores times it stay -infinity)
+  a.scale_log2 = fabsf(t->scale) * 1.4426950408889634f;
+  if (a.scale_log2 < FLT_MIN) a.scale_log2 = FLT_MIN;
+  a.flip = t->scale < 0.f ? 0x80008000u : 0u;
   a.workers = p.workers;
-  a.wave_rows = p.wave_rows;
   a.out_vec = c->d % 4 == 0 && ((uintptr_t)t->out & 7) == 0 && t->out_stride_row % 4 == 0 && t->out_stride_head % 4 == 0;
   char* ws = (char*)workspace;
   a.part = (TreePart*)ws;
@@ -144,11 +183,11 @@ extern "C" int spfa_tree_forward(const spfa_cache_t* c, const spfa_tree_t* t, vo
   a.pacc = (float*)(ws + p.part_bytes + 2 * p.state_bytes);
   const hipStream_t s = (hipStream_t)stream;
   if (c->dtype == SPFA_DTYPE_F16) {
-    if (c->code == SPFA_CODE_INT8) return tree_run<f16, SPFA_CODE_INT8>(a, p.rows_how, p.dp, p.rb, p.merge, s);
-    if (c->code == SPFA_CODE_E4M3) return tree_run<f16, SPFA_CODE_E4M3>(a, p.rows_how, p.dp, p.rb, p.merge, s);
-    return tree_run<f16, SPFA_CODE_NONE>(a, p.rows_how, p.dp, p.rb, p.merge, s);
+    if (c->code == SPFA_CODE_INT8) return tree_run<f16, SPFA_CODE_INT8>(a, p.shape, s);
+    if (c->code == SPFA_CODE_E4M3) return tree_run<f16, SPFA_CODE_E4M3>(a, p.shape, s);
+    return tree_run<f16, SPFA_CODE_NONE>(a, p.shape, s);
   }
-  if (c->code == SPFA_CODE_INT8) return tree_run<bf16, SPFA_CODE_INT8>(a, p.rows_how, p.dp, p.rb, p.merge, s);
-  if (c->code == SPFA_CODE_E4M3) return tree_run<bf16, SPFA_CODE_E4M3>(a, p.rows_how, p.dp, p.rb, p.merge, s);
-  return tree_run<bf16, SPFA_CODE_NONE>(a, p.rows_how, p.dp, p.rb, p.merge, s);
+  if (c->code == SPFA_CODE_INT8) return tree_run<bf16, SPFA_CODE_INT8>(a, p.shape, s);
+  if (c->code == SPFA_CODE_E4M3) return tree_run<bf16, SPFA_CODE_E4M3>(a, p.shape, s);
+  return tree_run<bf16, SPFA_CODE_NONE>(a, p.shape, s);
 }

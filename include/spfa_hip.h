@@ -460,7 +460,9 @@ typedef struct spfa_tree {
   float scale;
 } spfa_tree_t;
 
-/* The cache's dtype (SPFA_DTYPE_F16 or _BF16) is that of q and out too; d <= 256. */
+/* The cache's dtype (SPFA_DTYPE_F16 or _BF16) is that of q and out too; d <= 256; the strides of its
+ * pages and places (of keys, values and scales) are below 2^31 elements, and so is
+ * rows * heads_q / heads. */
 size_t spfa_tree_workspace_bytes(const spfa_cache_t* c, const spfa_tree_t* t);
 int spfa_tree_forward(const spfa_cache_t* c, const spfa_tree_t* t, void* workspace, size_t workspace_bytes,
                       void* stream);

@@ -506,6 +506,8 @@ class Run:
                     assert (np.abs(e) <= rel[has] + 2.0 ** -20).all()
 
 
+# places for many more tokens than the sequences have: calls over as much are worked on in larger tiles
+ROOM = dict(spare=33000, wide=16500)
 TREES = [  # dtype, code, d, page, kv heads, group, head_pages, ctx, nodes, mask
     (BF16, "none", 128, 16, 2, 4, True, [700], [1], "chain"),
     (F16, "none", 64, 32, 1, 8, True, [0, 31, 32, 33, 500], [1, 1, 1, 1, 1], "chain"),
@@ -545,6 +547,32 @@ def test_tree_attention(case):
     assert (other[..., r.d:] == 4.0).all()
 
 
+LARGE_TREES = [  # all with more than 192 rows per head
+    (F16, "none", 64, 16, 2, 8, True, [700, 0, 31, 128], [61, 40, 2, 50], "tree"),
+    (BF16, "none", 128, 16, 2, 8, False, [513, 90], [70, 33], "random"),
+    (BF16, "none", 96, 16, 2, 4, True, [300], [130], "chain"),
+    (F16, "none", 256, 16, 1, 4, True, [127, 1], [100, 29], "tree"),
+    (BF16, "int8", 64, 16, 1, 4, True, [400, 129], [64, 65], "random"),
+    (F16, "int8", 128, 16, 2, 7, False, [640, 5], [31, 33], "tree"),
+    (F16, "e4m3", 128, 16, 2, 8, True, [100, 3], [70, 10], "random"),
+    (BF16, "e4m3", 208, 16, 2, 3, True, [256], [128], "chain"),
+    (F16, "int8", 32, 16, 2, 5, True, [50, 0, 0], [70, 0, 60], "random"),
+    (BF16, "e4m3", 256, 16, 2, 1, True, [1000], [260], "tree"),
+]
+
+
+@pytest.mark.parametrize("case", LARGE_TREES, ids=lambda c: "%s_%s_d%d_%s_%d" % (str(c[0])[6:], c[1], c[2], c[9], max(c[7])))
+def test_tree_attention_of_many_rows(case):
+    r = Run(12, *case, front=1, behind=2, **ROOM)
+    out = torch.full(r.q.shape, 9.0, dtype=r.dt, device=DEV)
+    r.call(out)
+    r.check(out)
+    assert (out[:1] == 9.0).all() and (out[r.off[-1]:] == 9.0).all()
+    again = torch.full(r.q.shape, 9.0, dtype=r.dt, device=DEV)
+    r.call(again)
+    assert torch.equal(again, out)
+
+
 def test_tree_of_no_rows_no_pages_and_no_sequences():
     m = _mod("spfa_tree")
     r = Run(2, BF16, "none", 64, 16, 1, 2, True, [0, 0], [1, 2], "random")
@@ -566,11 +594,13 @@ def test_tree_of_no_rows_no_pages_and_no_sequences():
     assert not out.any()
 
 
+@pytest.mark.parametrize("nodes", [40, 130])
 @pytest.mark.parametrize("code,dt", [("none", BF16), ("none", F16), ("int8", BF16), ("e4m3", F16)])
-def test_tree_state_chains(code, dt):
+def test_tree_state_chains(code, dt, nodes):
     """Two caches one after the other on one (m, l, out), and scale of either sign."""
-    a = Run(3, dt, code, 64, 16, 2, 2, True, [300, 0, 40], [4, 3, 40], "random")
-    b = Run(4, dt, code, 64, 16, 2, 2, False, [129, 2, 0], [4, 3, 40], "tree")
+    room = ROOM if nodes > 100 else {}
+    a = Run(3, dt, code, 64, 16, 2, 2, True, [300, 0, 40], [4, 3, nodes], "random", **room)
+    b = Run(4, dt, code, 64, 16, 2, 2, False, [129, 2, 0], [4, 3, nodes], "tree", **room)
     b.q = a.q
     # the second one without its trees: whole contexts only
     b.mask.zero_()
@@ -647,11 +677,11 @@ def test_tree_bad_offsets_are_cut():
 
 
 @pytest.mark.parametrize("dt,code", [(BF16, "none"), (F16, "none"), (BF16, "e4m3"), (F16, "e4m3"), (BF16, "int8"), (F16, "int8")])
-@pytest.mark.parametrize("d,nodes", [(64, 20), (128, 6), (128, 40), (256, 9)])
+@pytest.mark.parametrize("d,nodes", [(64, 20), (128, 6), (128, 40), (256, 9), (64, 250), (128, 250), (256, 250)])
 def test_tree_infinities_reach_only_the_rows_that_attend_them(dt, code, d, nodes):
     """Drafted tokens whose keys or values hold infinities and NaN, attended by some nodes; places past
     the sequence and unused pages hold NaN throughout (Run fills them)."""
-    r = Run(7, dt, code, d, 16, 1, 2, True, [100, 3], [nodes, 4], "random")
+    r = Run(7, dt, code, d, 16, 1, 2, True, [100, 3], [nodes, 4], "random", **(ROOM if nodes > 100 else {}))
     kc, vc, ks, vs = r.cache
     rng = np.random.default_rng(9)
     sick_v = {0: [1, 2, nodes - 1], 1: [0, 3]}
