@@ -10,14 +10,20 @@
 // LPV lanes by DPP.  The angles of a token are the same for all its heads: a workgroup reduces them
 // once in fp64 (position * frequency / 2 pi, less its nearest whole number), takes sine and cosine
 // in fp32 and keeps them in LDS for the vectors of its tokens.
+//
+// Measured, 16384 tokens of 32 + 8 bf16 heads of 128: forward 69 us (4.9 TB/s, what a copy reaches),
+// gradients 128 us (3.9 TB/s; 193 registers leave two wavefronts per SIMD, fewer registers by one vector
+// on the way instead of two: 137 us, by spilling: 171) and 5 us for the weights' sum; one token 4 us.
 #include "spfa_serve.hpp"
 
 namespace spfa {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeBlocks = 1024;   // workgroups of a gradient call over both tensors
+constexpr int kRopeBatch = 2;       // vectors of a lane on the way at a time
 constexpr int kRopeLds = 32 * 1024; // bytes of cosines and sines a workgroup keeps at most
 
+enum { kNoWeights, kOwnWeights, kFloatWeights };  // of the vectors' type, of fp32
 struct RopeSide {
   const void* x;
   void* out;       // forward: the output; gradients: d_x
@@ -28,6 +34,9 @@ struct RopeSide {
   int64_t vectors;  // batch * tokens * heads
   int64_t chunks;   // of args.per_chunk vectors each
   int64_t blocks;   // workgroups that walk them
+  int32_t w_how;    // kNoWeights, ...
+  uint32_t magic;   // of heads (fast_div)
+  int32_t shift;
 };
 
 struct RopeArgs {
@@ -39,7 +48,34 @@ struct RopeArgs {
   float* partial;  // gradients: [blocks of both sides, d]
   float eps;
   int32_t d, rot, per_chunk;
-  int32_t wide_pos, interleaved, w_f32;
+  int32_t wide_pos, interleaved;
+  uint32_t half_magic;  // of rot / 2
+  int32_t half_shift;
+};
+
+// What a lane has of a vector, as loaded.
+template <typename T, int E, int NJ>
+struct RopeRow {
+  using Raw = std::conditional_t<E == 1, T, uint4v>;
+  Raw a[NJ], b[NJ];
+  __device__ __forceinline__ void load(const T* p, const int (&at_a)[NJ], const int (&at_b)[NJ]) {
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {  // (pieces that are not there are taken from the vector's start)
+      a[j] = *reinterpret_cast<const Raw*>(p + (at_a[j] < 0 ? 0 : at_a[j]));
+      b[j] = *reinterpret_cast<const Raw*>(p + (at_b[j] < 0 ? 0 : at_b[j]));
+    }
+  }
+  static __device__ __forceinline__ void piece(const Raw& raw, bool there, float (&f)[E]) {
+    if constexpr (E == 1) {
+      f[0] = there ? to_f32(raw) : 0.f;
+    } else {
+      uint4v x = raw;
+      const uint32_t mask = there ? 0xffffffffu : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] &= mask;
+      VecLay<T, 64>::unpack(x, f);
+    }
+  }
 };
 
 // A lane's elements: NJ pairs of pieces, piece j starting at a[j] and b[j] (-1: none).
@@ -107,9 +143,12 @@ __device__ __forceinline__ void turn(const RopeArgs& g, const float2* cs, int a,
   }
 }
 
-template <typename T, int LPV, int E, int NJ, bool GRAD>
+// R: vectors a slot of LPV lanes has on the way at a time.  The first of a chunk are asked for before the
+// angles are worked out.
+template <typename T, int LPV, int E, int NJ, int R, bool GRAD>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs g) {
   constexpr int kSlots = kRopeThreads / LPV;
+  using Row = RopeRow<T, E, NJ>;
   extern __shared__ __align__(16) char lds[];
   float2* cs = reinterpret_cast<float2*>(lds);
   const int tid = threadIdx.x, c = tid % LPV, slot = tid / LPV;
@@ -121,112 +160,136 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs g) {
 
   int a[NJ], b[NJ];
   piece_starts<E, NJ, LPV>(g, c, a, b);
-  // the weights of the lane's elements
+  // the weights of the lane's elements (single elements, or pieces of 16 bytes: host)
   float wa[NJ][E], wb[NJ][E], da[NJ][E], db[NJ][E];
 #pragma unroll
-  for (int j = 0; j < NJ; j++)
+  for (int j = 0; j < NJ; j++) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      auto weight = [&](int i) {
-        if (i < 0) return 0.f;
-        if (s.w == nullptr) return 1.f;
-        return g.w_f32 ? ((const float*)s.w)[i + e] : to_f32(((const T*)s.w)[i + e]);
-      };
-      wa[j][e] = weight(a[j]);
-      wb[j][e] = weight(b[j]);
+      wa[j][e] = wb[j][e] = 1.f;
       da[j][e] = db[j][e] = 0.f;
     }
+    const int ia = a[j] < 0 ? 0 : a[j], ib = b[j] < 0 ? 0 : b[j];
+    if (s.w_how == kOwnWeights) {
+      load_piece<T, E>((const T*)s.w + ia, wa[j]);
+      load_piece<T, E>((const T*)s.w + ib, wb[j]);
+    } else if (s.w_how == kFloatWeights) {
+      constexpr int F = E < 4 ? E : 4;
+#pragma unroll
+      for (int e = 0; e < E; e += F) {
+        load_piece<float, F>((const float*)s.w + ia + e, *reinterpret_cast<float(*)[F]>(&wa[j][e]));
+        load_piece<float, F>((const float*)s.w + ib + e, *reinterpret_cast<float(*)[F]>(&wb[j][e]));
+      }
+    }
+  }
 
   for (int64_t ch = blk; ch < s.chunks; ch += s.blocks) {
     const int64_t v0 = ch * g.per_chunk;
     const int n = (int)(s.vectors - v0 < g.per_chunk ? s.vectors - v0 : g.per_chunk);
-    const int64_t t0 = v0 / H;
+    // (64-bit divisions are hundreds of instructions)
+    const int64_t t0 = s.vectors < INT32_MAX ? (int64_t)fast_div((uint32_t)v0, s.magic, s.shift) : v0 / H;
     const int h0 = (int)(v0 - t0 * H);
-    const int64_t b0 = t0 / g.tokens, tok0 = t0 - b0 * g.tokens;
-    const int span = (h0 + n - 1) / H + 1;
-    __syncthreads();
-    for (int i = tid; i < span * half; i += kRopeThreads) {
-      const int k = i / half, p = i - k * half;
+    const int64_t b0 = t0 < g.tokens ? 0 : t0 < INT32_MAX ? (int64_t)((uint32_t)t0 / (uint32_t)g.tokens) : t0 / g.tokens;
+    const int64_t tok0 = t0 - b0 * g.tokens;
+    const int span = (int)fast_div((uint32_t)(h0 + n - 1), s.magic, s.shift) + 1;
+    Row x[R], y[GRAD ? R : 1];
+    T* to[R];
+    const float2* angles[R];
+    // the slot's vectors r * kSlots + slot from `first`; behind the chunk's last the last is taken instead
+    auto fetch = [&](int first) {
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const int vi = first + r * kSlots + slot;
+        const int hv = h0 + (vi < n ? vi : n - 1);
+        const int k = (int)fast_div((uint32_t)hv, s.magic, s.shift), h = hv - k * H;
+        int64_t bb = b0, tok = tok0 + k;
+        while (tok >= g.tokens) { tok -= g.tokens; bb++; }
+        angles[r] = cs + k * half;
+        to[r] = (T*)s.out + bb * s.os[0] + tok * s.os[1] + h * s.os[2];
+        x[r].load((const T*)s.x + bb * s.xs[0] + tok * s.xs[1] + h * s.xs[2], a, b);
+        if constexpr (GRAD) y[r].load((const T*)s.dy + bb * s.ds[0] + tok * s.ds[1] + h * s.ds[2], a, b);
+      }
+    };
+    // (what the lane's first angle needs is asked for ahead of the vectors)
+    auto angle = [&](int i, double& pos, float& freq) {
+      const int k = (int)fast_div((uint32_t)i, g.half_magic, g.half_shift), p = i - k * half;
       int64_t bb = b0, tok = tok0 + k;
       while (tok >= g.tokens) { tok -= g.tokens; bb++; }
-      const double pos = (double)load_index(g.positions, bb * g.position_stride + tok, g.wide_pos);
-      const double rev = pos * ((double)g.inv_freq[p] * 0.15915494309189533577);
+      pos = (double)load_index(g.positions, bb * g.position_stride + tok, g.wide_pos);
+      freq = g.inv_freq[p];
+    };
+    double pos = 0.0;
+    float freq = 0.f;
+    if (tid < span * half) angle(tid, pos, freq);
+    fetch(0);
+    __syncthreads();
+    for (int i = tid; i < span * half; i += kRopeThreads) {
+      if (i != tid) angle(i, pos, freq);
+      const double rev = pos * ((double)freq * 0.15915494309189533577);
       float sn, cn;
       sincospif(2.f * (float)(rev - rint(rev)), &sn, &cn);
       cs[i] = float2{cn, sn};
     }
     __syncthreads();
-    for (int vi = slot; vi < g.per_chunk; vi += kSlots) {
-      const bool ok = vi < n;
-      const int k = ok ? (h0 + vi) / H : 0, h = ok ? h0 + vi - k * H : 0;
-      int64_t bb = b0, tok = tok0 + k;
-      while (tok >= g.tokens) { tok -= g.tokens; bb++; }
-      const T* xr = (const T*)s.x + bb * s.xs[0] + tok * s.xs[1] + h * s.xs[2];
-      T* orow = (T*)s.out + bb * s.os[0] + tok * s.os[1] + h * s.os[2];
-      const float2* mine = cs + k * half;
-      float xa[NJ][E] = {}, xb[NJ][E] = {}, ya[NJ][E] = {}, yb[NJ][E] = {};
-      if (ok) {
+    for (int first = 0; first < g.per_chunk; first += R * kSlots) {
+      if (first > 0) fetch(first);
+#pragma unroll
+      for (int u = 0; u < R; u++) {
+        const bool ok = first + u * kSlots + slot < n;
+        float xa[NJ][E], xb[NJ][E];
+        float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-          if (a[j] >= 0) load_piece<T, E>(xr + a[j], xa[j]);
-          if (b[j] >= 0) load_piece<T, E>(xr + b[j], xb[j]);
-        }
-        if constexpr (GRAD) {
-          const T* dr = (const T*)s.dy + bb * s.ds[0] + tok * s.ds[1] + h * s.ds[2];
+          Row::piece(x[u].a[j], ok && a[j] >= 0, xa[j]);
+          Row::piece(x[u].b[j], ok && b[j] >= 0, xb[j]);
 #pragma unroll
-          for (int j = 0; j < NJ; j++) {
-            if (a[j] >= 0) load_piece<T, E>(dr + a[j], ya[j]);
-            if (b[j] >= 0) load_piece<T, E>(dr + b[j], yb[j]);
+          for (int e = 0; e < E; e++) ss = __builtin_fmaf(xa[j][e], xa[j][e], __builtin_fmaf(xb[j][e], xb[j][e], ss));
+        }
+        const float r = 1.f / sqrtf(group_sum<LPV>(ss) / (float)g.d + g.eps);
+        if constexpr (!GRAD) {
+          if (ok) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+#pragma unroll
+              for (int e = 0; e < E; e++) {
+                xa[j][e] *= r * wa[j][e];
+                xb[j][e] *= r * wb[j][e];
+              }
+              turn<E, 1>(g, angles[u], a[j], b[j], xa[j], xb[j]);
+              if (a[j] >= 0) store_piece<T, E>(to[u] + a[j], xa[j]);
+              if (b[j] >= 0) store_piece<T, E>(to[u] + b[j], xb[j]);
+            }
           }
-        }
-      }
-      float ss = 0.f;
-#pragma unroll
-      for (int j = 0; j < NJ; j++)
-#pragma unroll
-        for (int e = 0; e < E; e++) ss = __builtin_fmaf(xa[j][e], xa[j][e], __builtin_fmaf(xb[j][e], xb[j][e], ss));
-      const float r = 1.f / sqrtf(group_sum<LPV>(ss) / (float)g.d + g.eps);
-      if constexpr (!GRAD) {
-        if (ok) {
+        } else {
+          float ya[NJ][E], yb[NJ][E], dot = 0.f;
 #pragma unroll
           for (int j = 0; j < NJ; j++) {
+            Row::piece(y[u].a[j], ok && a[j] >= 0, ya[j]);
+            Row::piece(y[u].b[j], ok && b[j] >= 0, yb[j]);
+            turn<E, -1>(g, angles[u], a[j], b[j], ya[j], yb[j]);
 #pragma unroll
             for (int e = 0; e < E; e++) {
-              xa[j][e] *= r * wa[j][e];
-              xb[j][e] *= r * wb[j][e];
+              xa[j][e] *= r;  // n
+              xb[j][e] *= r;
+              da[j][e] = __builtin_fmaf(ya[j][e], xa[j][e], da[j][e]);
+              db[j][e] = __builtin_fmaf(yb[j][e], xb[j][e], db[j][e]);
+              ya[j][e] *= wa[j][e];
+              yb[j][e] *= wb[j][e];
+              dot = __builtin_fmaf(ya[j][e], xa[j][e], __builtin_fmaf(yb[j][e], xb[j][e], dot));
             }
-            turn<E, 1>(g, mine, a[j], b[j], xa[j], xb[j]);
-            if (a[j] >= 0) store_piece<T, E>(orow + a[j], xa[j]);
-            if (b[j] >= 0) store_piece<T, E>(orow + b[j], xb[j]);
           }
-        }
-      } else {
-        float dot = 0.f;
+          dot = group_sum<LPV>(dot) / (float)g.d;
+          if (ok) {
 #pragma unroll
-        for (int j = 0; j < NJ; j++) {
-          if (ok) turn<E, -1>(g, mine, a[j], b[j], ya[j], yb[j]);
+            for (int j = 0; j < NJ; j++) {
 #pragma unroll
-          for (int e = 0; e < E; e++) {
-            xa[j][e] *= r;  // n
-            xb[j][e] *= r;
-            da[j][e] = __builtin_fmaf(ya[j][e], xa[j][e], da[j][e]);
-            db[j][e] = __builtin_fmaf(yb[j][e], xb[j][e], db[j][e]);
-            ya[j][e] *= wa[j][e];
-            yb[j][e] *= wb[j][e];
-            dot = __builtin_fmaf(ya[j][e], xa[j][e], __builtin_fmaf(yb[j][e], xb[j][e], dot));
-          }
-        }
-        dot = group_sum<LPV>(dot) / (float)g.d;
-        if (ok) {
-#pragma unroll
-          for (int j = 0; j < NJ; j++) {
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-              ya[j][e] = r * (ya[j][e] - xa[j][e] * dot);
-              yb[j][e] = r * (yb[j][e] - xb[j][e] * dot);
+              for (int e = 0; e < E; e++) {
+                ya[j][e] = r * (ya[j][e] - xa[j][e] * dot);
+                yb[j][e] = r * (yb[j][e] - xb[j][e] * dot);
+              }
+              if (a[j] >= 0) store_piece<T, E>(to[u] + a[j], ya[j]);
+              if (b[j] >= 0) store_piece<T, E>(to[u] + b[j], yb[j]);
             }
-            if (a[j] >= 0) store_piece<T, E>(orow + a[j], ya[j]);
-            if (b[j] >= 0) store_piece<T, E>(orow + b[j], yb[j]);
           }
         }
       }
@@ -264,7 +327,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs g) {
   }
 }
 
-// d_w = the sum of the workgroups' parts: eight columns of a side per workgroup, 32 rows at a time.
+// d_w = the sum of the workgroups' parts: eight columns of a side per workgroup, 32 rows side by side and
+// eight of a lane's own on the way at a time.
 __global__ __launch_bounds__(256) void rope_weights_kernel(const float* partial, int64_t blocks_q, int64_t blocks_k,
                                                            int d, float* d_w_q, float* d_w_k) {
   __shared__ float acc[32][9];
@@ -272,12 +336,19 @@ __global__ __launch_bounds__(256) void rope_weights_kernel(const float* partial,
   if (to == nullptr) return;
   const int64_t first = blockIdx.y ? blocks_q : 0, n = blockIdx.y ? blocks_k : blocks_q;
   const int col = threadIdx.x % 8, row = threadIdx.x / 8, i = blockIdx.x * 8 + col;
+  const float* from = partial + first * d + (i < d ? i : 0);
   float x = 0.f;
-  if (i < d)
-    for (int64_t r = row; r < n; r += 32) x += partial[(first + r) * d + i];
+  for (int64_t r = row; r < n; r += 8 * 32) {
+    float y[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) y[u] = from[(r + 32 * u < n ? r + 32 * u : r) * d];
+#pragma unroll
+    for (int u = 0; u < 8; u++) x += r + 32 * u < n ? y[u] : 0.f;
+  }
   acc[row][col] = x;
   __syncthreads();
   if (row == 0 && i < d) {
+#pragma unroll
     for (int r = 1; r < 32; r++) x += acc[r][col];
     to[i] = x;
   }
@@ -313,6 +384,7 @@ int rope_launch(RopeArgs& g, hipStream_t stream) {
   g.per_chunk = rope_chunk(g, kSlots, min_heads, &lds);
   const int64_t all = g.side[0].vectors + g.side[1].vectors;
   for (RopeSide& s : g.side) {
+    fast_divider((int32_t)s.heads, &s.magic, &s.shift);
     s.chunks = (s.vectors + g.per_chunk - 1) / g.per_chunk;
     s.blocks = s.chunks;
     if (GRAD) {
@@ -327,7 +399,12 @@ int rope_launch(RopeArgs& g, hipStream_t stream) {
   const size_t need = GRAD ? (size_t)4 * g.d * sizeof(float) : 0;
   if (lds < need) lds = need;
   const int64_t blocks = g.side[0].blocks + g.side[1].blocks;
-  rope_kernel<T, LPV, E, NJ, GRAD><<<dim3((unsigned)blocks), dim3(kRopeThreads), lds, stream>>>(g);
+  if constexpr (E > 1)
+    if (g.per_chunk >= kRopeBatch * kSlots) {
+      rope_kernel<T, LPV, E, NJ, kRopeBatch, GRAD><<<dim3((unsigned)blocks), dim3(kRopeThreads), lds, stream>>>(g);
+      return launch_status();
+    }
+  rope_kernel<T, LPV, E, NJ, 1, GRAD><<<dim3((unsigned)blocks), dim3(kRopeThreads), lds, stream>>>(g);
   return launch_status();
 }
 
@@ -390,6 +467,8 @@ bool rope_args(const spfa_rope_t* p, const spfa_heads_t* const (&out)[2], const 
     s.x = x[i].data;
     s.out = out[i]->data;
     s.w = w[i];
+    s.w_how = w[i] == nullptr ? kNoWeights : p->w_dtype == p->dtype ? kOwnWeights : kFloatWeights;
+    *aligned = *aligned && ((uintptr_t)w[i] & 15) == 0;
     set_strides(s.xs, x[i]);
     set_strides(s.os, *out[i]);
     *aligned = *aligned && heads_aligned(x[i], size, p->batch > 1) && heads_aligned(*out[i], size, p->batch > 1);
@@ -411,7 +490,7 @@ bool rope_args(const spfa_rope_t* p, const spfa_heads_t* const (&out)[2], const 
   g.rot = (int32_t)p->rot;
   g.wide_pos = p->position_bytes == 8;
   g.interleaved = p->interleaved != 0;
-  g.w_f32 = p->w_dtype == SPFA_DTYPE_F32;
+  if (g.rot > 0) fast_divider(g.rot / 2, &g.half_magic, &g.half_shift);
   return true;
 }
 

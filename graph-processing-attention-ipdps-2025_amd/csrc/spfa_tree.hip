@@ -26,16 +26,6 @@ struct TreePlan {
 
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// p / d for p < 2^31 as (p * magic >> 32) >> shift (shift < 0: d is 1).  With s the bits of d - 1 and
-// magic = ceil(2^(31 + s) / d) < 2^32, p * magic exceeds p * 2^(31 + s) / d by less than
-// p / 2^31 * 2^(31 + s) / d, too little to reach the next whole quotient.
-void tree_divider(int32_t d, uint32_t* magic, int32_t* shift) {
-  int s = 0;
-  while (((int64_t)1 << s) < d) s++;
-  *shift = s - 1;
-  *magic = s == 0 ? 0u : (uint32_t)((((uint64_t)1 << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d);
-}
-
 int tree_check(const spfa_cache_t* c, const spfa_tree_t* t) {
   if (c == nullptr || t == nullptr) return SPFA_ERR_BAD_ARG;
   if (c->d < 1 || c->d > 256) return SPFA_ERR_EMB_TOO_LARGE;
@@ -166,9 +156,9 @@ extern "C" int spfa_tree_forward(const spfa_cache_t* c, const spfa_tree_t* t, vo
   a.d = (int32_t)c->d;
   a.page_size = (int32_t)c->page_size;
   a.max_len = !keys ? 0 : t->table_width < kMaxPositions / c->page_size ? (int32_t)(t->table_width * c->page_size) : (int32_t)kMaxPositions;
-  tree_divider(a.page_size, &a.page_magic, &a.page_shift);
-  tree_divider(a.group, &a.group_magic, &a.group_shift);
-  tree_divider(p.shape.rows(), &a.tile_magic, &a.tile_shift);
+  fast_divider(a.page_size, &a.page_magic, &a.page_shift);
+  fast_divider(a.group, &a.group_magic, &a.group_shift);
+  fast_divider(p.shape.rows(), &a.tile_magic, &a.tile_shift);
   // the kernels look for the largest score before they scale it: a negative scale becomes the queries'
   // sign, and zero the smallest number there is (masked scores times it stay -infinity)
   a.scale_log2 = fabsf(t->scale) * 1.4426950408889634f;

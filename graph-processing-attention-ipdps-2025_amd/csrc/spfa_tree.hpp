@@ -60,7 +60,7 @@ struct TreeArgs {
   int64_t mask_words;
   int64_t rows, pages;
   int32_t heads, group, n_seqs, d, page_size;
-  // p / size = (p * magic >> 32) >> shift for p < 2^31; shift < 0: p (host: tree_divider)
+  // p / size = (p * magic >> 32) >> shift for p < 2^31; shift < 0: p (host: fast_divider)
   uint32_t page_magic, group_magic, tile_magic;  // of page_size, group, rows of an item
   int32_t page_shift, group_shift, tile_shift;
   int32_t max_len;  // positions the page table covers, cut to 32 bits
@@ -75,7 +75,6 @@ struct TreeArgs {
 };
 
 // (64-bit divisions are hundreds of dependent instructions: none on the way of ordinary sizes)
-__device__ __forceinline__ uint32_t tree_div(uint32_t p, uint32_t magic, int shift) { return shift < 0 ? p : __umulhi(p, magic) >> shift; }
 __device__ __forceinline__ int64_t tree_div64(int64_t a, int64_t b) {
   if (((uint64_t)a | (uint64_t)b) >> 32) return a / b;
   return (int64_t)((uint32_t)a / (uint32_t)b);
@@ -96,7 +95,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& g, int s, int M) {
   q.ctx = ctx < 0 ? 0 : ctx;
   const int64_t len = (int64_t)q.ctx + q.n;
   q.len = (int)(len < g.max_len ? len : g.max_len);
-  q.tiles = (int)tree_div((uint32_t)(q.n * g.group + M - 1), g.tile_magic, g.tile_shift);  // (host: rows * group stays below 2^31)
+  q.tiles = (int)fast_div((uint32_t)(q.n * g.group + M - 1), g.tile_magic, g.tile_shift);  // (host: rows * group stays below 2^31)
   q.nblk = q.len <= kTreeBlock ? 1 : (q.len + kTreeBlock - 1) / kTreeBlock;
   return q;
 }
@@ -357,7 +356,7 @@ struct TreeQueries {
     // (lanes without a row work on the tile's last one; what they get is not written)
     const int r = first_row + c < it.live_rows ? first_row + c : it.live_rows - 1;
     const int rr = it.tile0 + r;
-    node = (int)tree_div((uint32_t)rr, a.group_magic, a.group_shift);
+    node = (int)fast_div((uint32_t)rr, a.group_magic, a.group_shift);
     const int gi = rr - node * a.group;
     const T* qp = (const T*)a.q + (int64_t)(it.sq.row0 + node) * a.qs_row + (int64_t)(it.head * a.group + gi) * a.qs_head;
     bits = a.mask + (int64_t)(it.sq.row0 + node) * a.mask_words;
@@ -439,14 +438,14 @@ struct TreeKeys {
     s_page = uniform(a.ks_page), s_slot = uniform(a.ks_slot), u_page = uniform(a.vs_page), u_slot = uniform(a.vs_slot);
     page_size = uniform(a.page_size), magic = uniform(a.page_magic), shift = uniform(a.page_shift), pages = uniform((int)a.pages);
     lim = uniform(it.sq.len < t_end * 32 ? it.sq.len : t_end * 32);
-    last = lim > 0 ? tree_div(lim - 1, magic, shift) : 0;
+    last = lim > 0 ? fast_div(lim - 1, magic, shift) : 0;
     off = off_lds;
     ks = vs = 0.f;
   }
   // asks for the page of this lane's key of a tile
   __device__ __forceinline__ void look_up(int t) {
     const uint32_t p = (uint32_t)(t * 32 + (lane_id() & 31));
-    const uint32_t q = tree_div(p, magic, shift);
+    const uint32_t q = fast_div(p, magic, shift);
     place = p < lim ? p - q * page_size : kNowhere;
     page = table[q < last ? q : last];  // (past the end the last page's entry: no branch around the load)
   }
@@ -803,7 +802,7 @@ __device__ __forceinline__ void tree_join(const TreeArgs& g, const TreeWalk& it,
     }
     if (whole) {
       const int rr = it.tile0 + r;
-      const int nd = (int)tree_div((uint32_t)rr, g.group_magic, g.group_shift), gi = rr - nd * g.group;
+      const int nd = (int)fast_div((uint32_t)rr, g.group_magic, g.group_shift), gi = rr - nd * g.group;
       const TreeWeights tw = tree_weights(g, it.sq.row0 + nd, it.head * g.group + gi, mx, lt);
 #pragma unroll
       for (int e = 0; e < EB; e++) tree_store<T, 4>(g, it.sq.row0 + nd, it.head * g.group + gi, 4 * (8 * e + sub), tw, x[e]);
@@ -1245,7 +1244,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs g, int M) {
     }
     if (sub == 0 && r < live_rows) {
       const int rr = tile0 + r;
-      const int nd = (int)tree_div((uint32_t)rr, g.group_magic, g.group_shift), gi = rr - nd * g.group;
+      const int nd = (int)fast_div((uint32_t)rr, g.group_magic, g.group_shift), gi = rr - nd * g.group;
       const TreeWeights tw = tree_weights(g, sq.row0 + nd, part.head * g.group + gi, m, l);
 #pragma unroll
       for (int i = 0; i < N / V; i++) {

@@ -127,6 +127,43 @@ def test_rope_forward_and_gradients(case):
     assert torch.equal(dqo, dq) and torch.equal(dko, dk) and torch.equal(dw2[0], dw[0]) and torch.equal(dw2[1], dw[1])
 
 
+@pytest.mark.parametrize("case,batch", [
+    ((BF16, 11, 6, 2, 128, 128, False, BF16, True, False), 901),   # more rows of a batch than tokens in a workgroup's share
+    ((F32, 4713, 12, 2, 64, 32, True, F32, True, False), 1),
+    ((F16, 2100, 3, 1, 33, 10, False, F16, False, False), 2),
+    ((BF16, 1, 5, 1, 256, 64, False, F32, False, False), 6007),    # one token of each
+], ids=["bf16", "f32", "odd", "steps"])
+def test_rope_of_many_vectors(case, batch):
+    """Calls that fill the device: workgroups with several rounds and shares, and weights at odd addresses."""
+    dt, tokens, hq, hk, d, rot, inter, wdt, fused, _ = case
+    q, k, w, pos, f = _rope_inputs(case, 8, batch)
+    m = _mod("spfa_rope")
+    qo, ko = torch.empty(q.shape, dtype=dt, device=DEV), torch.empty(k.shape, dtype=dt, device=DEV)
+    m.forward(q, k, *w, pos, f, qo, ko, 1e-5, inter)
+    g = _gen(9)
+    dqo, dko = [torch.randn(x.shape, generator=g, device=DEV).to(dt) for x in (q, k)]
+    dq, dk = torch.empty_like(dqo), torch.empty_like(dko)
+    dw = [torch.empty(d, device=DEV) for _ in range(2)]
+    m.backward(q, k, *w, pos, f, dqo, dko, dq, dk, *dw, 1e-5, inter)
+    p, fr = pos.flatten().cpu().numpy(), np64(f)
+    flat = lambda x: np64(x).reshape(batch * tokens, -1, d)
+    for x, y, dy, dx, ww, dww, heads in ((q, qo, dqo, dq, w[0], dw[0], hq), (k, ko, dko, dk, w[1], dw[1], hk)):
+        want = sv.norm_rope(flat(x), _ones(ww, d), p, fr, 1e-5, inter)
+        _close(y.reshape(want.shape), want, HALF[dt] * np.abs(want) + TINY[dt] + (d / 2 + 28) * U * _pair_size(want, rot, inter) * 1.5, "forward")
+        gx, gw, sx, sw = sv.norm_rope_backward(flat(x), _ones(ww, d), p, fr, 1e-5, inter, flat(dy))
+        _close(dx.reshape(gx.shape), gx, HALF[dt] * np.abs(gx) + TINY[dt] + (d + 60) * U * sx, "gradient")
+        _close(dww, gw, (d + 60 + batch * tokens * heads) * U * sw + TINY[F32], "weights' gradient")
+    # weights that do not start at a multiple of 16 bytes
+    odd = [torch.cat((x[:1], x))[1:] for x in w]
+    q2, k2 = torch.empty_like(qo), torch.empty_like(ko)
+    m.forward(q, k, *odd, pos, f, q2, k2, 1e-5, inter)
+    for y, y2 in ((qo, q2), (ko, k2)):
+        # (other lanes sum the squares: either is within the bound above of the exact value)
+        want = np64(y).reshape(batch * tokens, -1, d)
+        _close(y2.reshape(want.shape), want, 2 * HALF[dt] * np.abs(want) * 1.01 + 2 * TINY[dt]
+               + (d + 56) * U * _pair_size(want, rot, inter) * 1.6, "weights at an odd address")
+
+
 def test_rope_batches_positions_and_empty_sides():
     m = _mod("spfa_rope")
     case = (BF16, 3, 2, 1, 64, 64, False, BF16, True, False)
