@@ -5,7 +5,10 @@
 // Both directions only move rows: every element is loaded once and stored once, in 16-byte pieces of
 // the wider side where the tensors allow it, a row by LPV lanes, the row's largest absolute value
 // found among them by DPP.  Rows are dealt to lane groups in the order in which they lie next to
-// each other in the tensor outside the cache.
+// each other in the tensor outside the cache.  Measured: 32768 e4m3 tokens of 8 heads of 128 to bf16
+// 31 us (6.4 TB/s read and written), 2048 bf16 tokens written in 5 us; one token each of four sequences 3 us.
+#include <type_traits>
+
 #include "spfa_serve.hpp"
 
 namespace spfa {
@@ -26,32 +29,44 @@ struct CacheArgs {
   const void* slots;
   int64_t tokens, heads, page_size, n_slots;
   int32_t d, wide, token_fast;
+  int32_t small;  // rows and slots are below 2^31: rows and pages by fast_div
+  uint32_t row_magic, page_magic;
+  int32_t row_shift, page_shift;
 };
 
-// The quotient of two floats, x * top / amax, as the code nearest to its exact value.  In 32 bits
-// the quotient of two 16-bit floats is on the right side of every border between two codes (its
-// exact value is either on the border, and comes out exactly, or at least 2^-19 of itself away); that of
-// two fp32 values needs 64, and for e4m3 a rounding to odd on the way through fp32.
+// x * top / amax as the code nearest to its exact value, by one division per row.  Against a border
+// between two codes, a number of few bits, the exact quotient is either equal or at least 2^-19 of itself
+// away for 16-bit floats (2^-34 for fp32, worked on in 64 bits).  x * top is exact and its product with
+// the rounded reciprocal is off by less than 2 units of the last place, so dropping the last 2 (12) bits by
+// rounding restores what lies on a border and takes nothing across one.
 template <typename T, int CODE>
-__device__ __forceinline__ float quotient(float x, float amax) {
-  constexpr float top = CODE == SPFA_CODE_INT8 ? 127.f : 448.f;
-  if constexpr (sizeof(T) == 2) {
-    // (bf16 reaches where x * top would overflow: scaled down, which changes no quotient)
-    const float s = amax > 0x1p100f ? 0x1p-64f : 1.f;
-    const float y = (x * s) * top / (amax * s);
-    return CODE == SPFA_CODE_INT8 ? rintf(y) : y;
-  } else {
-    const double y = (double)x * (double)top / (double)amax;
-    if (CODE == SPFA_CODE_INT8) return (float)rint(y);
-    const float f = (float)y;
-    if ((double)f == y || y != y) return f;
-    // truncated, and its last bit set: still between the same two codes, never on a border
-    uint32_t u = __builtin_bit_cast(uint32_t, f);
-    if (fabs((double)f) > fabs(y)) u -= 1;
-    u |= 1;
-    return __builtin_bit_cast(float, u);
+struct Quotient {
+  static constexpr float kTop = CODE == SPFA_CODE_INT8 ? 127.f : 448.f;
+  using W = std::conditional_t<sizeof(T) == 2, float, double>;
+  W by;
+  float s;
+  __device__ __forceinline__ explicit Quotient(float amax) {
+    // (bf16 reaches where x * top would overflow, and the reciprocal: scaled, which changes no quotient)
+    s = sizeof(T) == 4 ? 1.f : amax > 0x1p100f ? 0x1p-64f : amax < 0x1p-60f ? 0x1p64f : 1.f;
+    by = (W)1 / ((W)amax * (W)s);
   }
-}
+  __device__ __forceinline__ float operator()(float x) const {
+    if constexpr (sizeof(T) == 2) {
+      const float y = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, (x * s) * kTop * by) + 2u) & ~3u);
+      return CODE == SPFA_CODE_INT8 ? rintf(y) : y;
+    } else {
+      const double y = __builtin_bit_cast(double, (__builtin_bit_cast(uint64_t, (double)x * (double)kTop * by) + 0x800u) & ~(uint64_t)0xfff);
+      if (CODE == SPFA_CODE_INT8) return (float)rint(y);
+      const float f = (float)y;
+      if ((double)f == y || y != y) return f;
+      // truncated, and its last bit set: still between the same two codes, never on a border
+      uint32_t u = __builtin_bit_cast(uint32_t, f);
+      if (fabs((double)f) > fabs(y)) u -= 1;
+      u |= 1;
+      return __builtin_bit_cast(float, u);
+    }
+  }
+};
 
 // Codes of four elements, a byte each.
 template <int CODE>
@@ -101,7 +116,12 @@ __device__ __forceinline__ CacheRow cache_row(const CacheArgs& g, const CacheSid
   CacheRow r{0, 0, 0, false};
   if (row >= g.tokens * g.heads) return r;
   int64_t t, h;
-  if (g.token_fast) {
+  // (64-bit divisions are hundreds of instructions)
+  if (g.small) {
+    const int64_t big = fast_div((uint32_t)row, g.row_magic, g.row_shift), rest = row - big * (g.token_fast ? g.tokens : g.heads);
+    t = g.token_fast ? rest : big;
+    h = g.token_fast ? big : rest;
+  } else if (g.token_fast) {
     h = row / g.tokens;
     t = row - h * g.tokens;
   } else {
@@ -110,7 +130,7 @@ __device__ __forceinline__ CacheRow cache_row(const CacheArgs& g, const CacheSid
   }
   const int64_t slot = load_index(g.slots, t, g.wide);
   if (slot < 0 || slot >= g.n_slots) return r;
-  const int64_t page = slot / g.page_size, place = slot - page * g.page_size;
+  const int64_t page = g.small ? (int64_t)fast_div((uint32_t)slot, g.page_magic, g.page_shift) : slot / g.page_size, place = slot - page * g.page_size;
   r.outside = t * s.token + h * s.head;
   r.inside = page * s.page + place * s.slot + h * s.chead;
   r.scale = page * s.spage + place * s.sslot + h * s.shead;
@@ -118,14 +138,14 @@ __device__ __forceinline__ CacheRow cache_row(const CacheArgs& g, const CacheSid
   return r;
 }
 
-// E elements of a lane's piece (one, or 16: whole 16-byte pieces of codes), a lane's NJ pieces LPV
-// pieces apart.
+// E elements of a lane's piece, a lane's NJ pieces LPV pieces apart.
 template <typename T, int CODE, int LPV, int E, int NJ, bool WRITE>
 __global__ __launch_bounds__(kCacheThreads) void cache_kernel(CacheArgs g) {
   constexpr int kSlots = kCacheThreads / LPV;
   const int c = threadIdx.x % LPV;
   const CacheSide& s = g.side[blockIdx.y];
   const int64_t rows = g.tokens * g.heads;
+  typedef uint32_t Codes __attribute__((ext_vector_type(E < 4 ? 1 : E / 4)));
   constexpr int P = E == 1 ? 1 : 16 / (int)sizeof(T);  // elements of a 16-byte piece of rows
   for (int64_t r0 = (int64_t)blockIdx.x * kSlots; r0 < rows; r0 += (int64_t)gridDim.x * kSlots) {
     const CacheRow r = cache_row(g, s, r0 + threadIdx.x / LPV);
@@ -171,24 +191,24 @@ __global__ __launch_bounds__(kCacheThreads) void cache_kernel(CacheArgs g) {
         }
         const float amax = __builtin_bit_cast(float, group_max<LPV>(top));
         if (r.ok) {
-          const float div = amax == 0.f ? 1.f : amax;
+          const Quotient<T, CODE> code(amax == 0.f ? 1.f : amax);
 #pragma unroll
           for (int j = 0; j < NJ; j++) {
             const int i0 = (c + j * LPV) * E;
             if (i0 >= g.d) continue;
             if constexpr (E == 1) {
-              const float q[4] = {quotient<T, CODE>(f[j][0], div), 0.f, 0.f, 0.f};
+              const float q[4] = {code(f[j][0]), 0.f, 0.f, 0.f};
               y[i0] = (uint8_t)pack_codes<CODE>(q);
             } else {
-              uint4v w;
+              Codes w;
 #pragma unroll
-              for (int k = 0; k < 4; k++) {
+              for (int k = 0; k < E / 4; k++) {
                 float q[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) q[e] = quotient<T, CODE>(f[j][4 * k + e], div);
+                for (int e = 0; e < 4; e++) q[e] = code(f[j][4 * k + e]);
                 w[k] = pack_codes<CODE>(q);
               }
-              *reinterpret_cast<uint4v*>(y + i0) = w;
+              *reinterpret_cast<Codes*>(y + i0) = w;
             }
           }
           if (c == 0) s.scale[r.scale] = amax / (CODE == SPFA_CODE_INT8 ? 127.f : 448.f);
@@ -204,10 +224,10 @@ __global__ __launch_bounds__(kCacheThreads) void cache_kernel(CacheArgs g) {
             unpack_codes<CODE>(y[i0], q);
             x[i0] = from_f32<T>(q[0] * sc);
           } else {
-            const uint4v w = *reinterpret_cast<const uint4v*>(y + i0);
+            const Codes w = *reinterpret_cast<const Codes*>(y + i0);
             float f[E];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
+            for (int k = 0; k < E / 4; k++) {
               float q[4];
               unpack_codes<CODE>(w[k], q);
 #pragma unroll
@@ -251,11 +271,19 @@ int cache_launch(const CacheArgs& g, bool aligned, hipStream_t stream) {
     return dim3((unsigned)(n < (1 << 22) ? n : (1 << 22)), 2);  // (a grid holds fewer than 2^32 work items)
   };
   const dim3 block(kCacheThreads);
+  // A lane's piece is 16 bytes of codes, or of the rows where there are no codes (32768 tokens of 8 heads of
+  // 128 appended and read back: bf16 89 us, fp32 193, 101 and 489 with 16 elements).  fp32 rows with four
+  // elements a lane come back faster by 2 us of 20, but are written in 28 us instead of 16 (15003 tokens of 5
+  // heads of 80): each lane has the row's place and reciprocal to work out.
+  constexpr int E = CODE == SPFA_CODE_NONE ? 16 / (int)sizeof(T) : 16;
+  const int lanes = g.d / E;
   if (aligned && g.d % 16 == 0) {
-    if (g.d <= 64) cache_kernel<T, CODE, 4, 16, 1, WRITE><<<grid(4), block, 0, stream>>>(g);
-    else if (g.d <= 128) cache_kernel<T, CODE, 8, 16, 1, WRITE><<<grid(8), block, 0, stream>>>(g);
-    else if (g.d <= 256) cache_kernel<T, CODE, 16, 16, 1, WRITE><<<grid(16), block, 0, stream>>>(g);
-    else cache_kernel<T, CODE, 64, 16, 1, WRITE><<<grid(64), block, 0, stream>>>(g);
+    if (lanes <= 4) cache_kernel<T, CODE, 4, E, 1, WRITE><<<grid(4), block, 0, stream>>>(g);
+    else if (lanes <= 8) cache_kernel<T, CODE, 8, E, 1, WRITE><<<grid(8), block, 0, stream>>>(g);
+    else if (lanes <= 16) cache_kernel<T, CODE, 16, E, 1, WRITE><<<grid(16), block, 0, stream>>>(g);
+    else if (lanes <= 32) cache_kernel<T, CODE, 32, E, 1, WRITE><<<grid(32), block, 0, stream>>>(g);
+    else if (lanes <= 64) cache_kernel<T, CODE, 64, E, 1, WRITE><<<grid(64), block, 0, stream>>>(g);
+    else if constexpr (E < 16) cache_kernel<T, CODE, 64, E, 16 / E, WRITE><<<grid(64), block, 0, stream>>>(g);
   } else if (g.d <= 256) {
     cache_kernel<T, CODE, 64, 1, 4, WRITE><<<grid(64), block, 0, stream>>>(g);
   } else {
@@ -307,6 +335,11 @@ int cache_run(const spfa_cache_t* c, const spfa_heads_t* k, const spfa_heads_t* 
   g.wide = slot_bytes == 8;
   // rows in the order in which they follow each other in the tensor outside the cache
   g.token_fast = k->stride_token < k->stride_head;
+  g.small = tokens * c->heads < INT32_MAX && g.n_slots < INT32_MAX;
+  if (g.small) {
+    fast_divider((int32_t)(g.token_fast ? tokens : c->heads), &g.row_magic, &g.row_shift);
+    fast_divider((int32_t)c->page_size, &g.page_magic, &g.page_shift);
+  }
   switch (c->dtype) {
     case SPFA_DTYPE_F32: return cache_code<float, WRITE>(g, c->code, aligned, (hipStream_t)stream);
     case SPFA_DTYPE_F16: return cache_code<f16, WRITE>(g, c->code, aligned, (hipStream_t)stream);

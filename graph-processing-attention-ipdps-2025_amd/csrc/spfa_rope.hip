@@ -14,6 +14,8 @@
 // Measured, 16384 tokens of 32 + 8 bf16 heads of 128: forward 69 us (4.9 TB/s, what a copy reaches),
 // gradients 128 us (3.9 TB/s; 193 registers leave two wavefronts per SIMD, fewer registers by one vector
 // on the way instead of two: 137 us, by spilling: 171) and 5 us for the weights' sum; one token 4 us.
+#include <type_traits>
+
 #include "spfa_serve.hpp"
 
 namespace spfa {
