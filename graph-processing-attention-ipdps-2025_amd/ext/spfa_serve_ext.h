@@ -26,11 +26,21 @@ inline spfa_heads_t heads_of(const torch::Tensor& t) {
   return spfa_heads_t{t.data_ptr(), n == 4 ? stride_of(t, 0) : 0, stride_of(t, n - 3), stride_of(t, n - 2)};
 }
 
-// An output may be the very tensor that it is computed from; no other overlap.
-inline void check_output(const torch::Tensor& out, const char* name, std::initializer_list<torch::Tensor> others) {
+// An output overlaps neither itself nor other tensors of the call, except that it may be the very tensor
+// it is computed from row by row (`own`).
+inline void check_output(const torch::Tensor& out, const char* name, std::initializer_list<torch::Tensor> others,
+                         std::initializer_list<torch::Tensor> own = {}) {
   TORCH_CHECK(at::has_internal_overlap(out) != at::MemOverlap::Yes, name, " must not overlap itself");
-  for (const torch::Tensor& x : others)
-    TORCH_CHECK(at::get_overlap_status(out, x) != at::MemOverlapStatus::Partial, name, " partly overlaps another tensor of the call");
+  for (const torch::Tensor& x : others) {
+    const auto o = at::get_overlap_status(out, x);
+    TORCH_CHECK(o != at::MemOverlapStatus::Partial && o != at::MemOverlapStatus::Full &&
+                    (out.numel() == 0 || x.numel() == 0 || out.data_ptr() != x.data_ptr()),
+                name, " overlaps another tensor of the call");
+  }
+  for (const torch::Tensor& x : own)
+    TORCH_CHECK(at::get_overlap_status(out, x) != at::MemOverlapStatus::Partial &&
+                    (out.numel() == 0 || out.data_ptr() != x.data_ptr() || out.strides() == x.strides()),
+                name, " partly overlaps another tensor of the call");
 }
 
 inline int32_t serve_dtype(const torch::Tensor& t, const char* name) {

@@ -71,10 +71,9 @@ torch::Tensor spfa_tree_forward_py(torch::Tensor q, torch::Tensor k_cache, torch
   t.m = m.has_value() ? (float*)m->data_ptr() : nullptr;
   t.l = l.has_value() ? (float*)l->data_ptr() : nullptr;
   t.scale = scale.has_value() ? (float)*scale : 1.f / std::sqrt((float)c.d);
-  spfa_ext::check_output(out, "out", {k_cache, v_cache, page_table, ctx_lens, q_offsets});
   // (a row of q is read by every workgroup that has a part of its keys, so out cannot take its place)
-  TORCH_CHECK(out.numel() == 0 || out.data_ptr() != q.data_ptr(), "out must not be q");
-  TORCH_CHECK(at::get_overlap_status(out, q) != at::MemOverlapStatus::Partial, "out partly overlaps another tensor of the call");
+  spfa_ext::check_output(out, "out", {q, k_cache, v_cache, page_table, ctx_lens, q_offsets});
+  if (m.has_value()) spfa_ext::check_output(*m, "m", {*l});
   c10::DeviceGuard guard(q.device());
   torch::Tensor ws = spfa_ext::make_workspace(spfa_tree_workspace_bytes(&c, &t), q);
   spfa_ext::raise_on_error(spfa_tree_forward(&c, &t, ws.data_ptr(), (size_t)ws.numel(), spfa_ext::current_stream(q)));

@@ -807,6 +807,38 @@ def test_tree_and_cache_offsets_beyond_32_bits():
     assert torch.equal(out, want)
 
 
+def test_outputs_that_are_other_tensors_of_the_call_are_refused():
+    """An output in place of its own input is one thing, in place of another tensor a race."""
+    q, k = [torch.randn(6, 2, 64, generator=_gen(i), device=DEV).to(BF16) for i in (1, 2)]
+    w, f, pos = torch.ones(64, dtype=BF16, device=DEV), torch.ones(32, device=DEV), torch.arange(6, device=DEV)
+    m = _mod("spfa_rope")
+    qo, ko, dw = torch.empty_like(q), torch.empty_like(k), torch.empty(64, device=DEV)
+    for a, b in ((k, ko), (qo, q), (k, q), (qo, qo)):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            m.forward(q, k, w, w, pos, f, a, b)
+        with pytest.raises(RuntimeError, match="overlaps"):
+            m.backward(q, k, w, w, pos, f, q, k, a, b, None, None)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        m.backward(q, k, w, w, pos, f, q, k, qo, ko, dw, dw)
+    flat = torch.randn(6, 2, 64, generator=_gen(3), device=DEV).to(BF16)
+    with pytest.raises(RuntimeError, match="overlaps"):  # the same memory in another order
+        m.forward(flat, k, w, w, pos, f, flat.view(2, 6, 64).transpose(0, 1), ko)
+    c = _mod("spfa_cache")
+    kc = torch.zeros(2, 16, 2, 64, dtype=torch.int8, device=DEV)
+    ks = torch.zeros(2, 16, 2, device=DEV)
+    slots = torch.arange(6, device=DEV)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        c.write(q, k, slots, kc, kc, ks, ks.clone())
+    with pytest.raises(RuntimeError, match="overlaps"):
+        c.write(q, k, slots, kc, kc.clone(), ks, ks)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        c.read(kc, kc.clone(), slots, qo, qo, ks, ks.clone())
+    r = Run(1, BF16, "none", 64, 16, 2, 2, True, [20], [3], "tree")
+    out, ml = torch.empty(r.q.shape, dtype=BF16, device=DEV), torch.zeros(3, 4, device=DEV)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        r.call(out, m=ml, l=ml)
+
+
 def test_tree_refusals():
     m = _mod("spfa_tree")
     r = Run(1, BF16, "int8", 64, 16, 2, 2, True, [20], [3], "tree")
