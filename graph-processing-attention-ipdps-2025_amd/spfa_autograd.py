@@ -120,6 +120,7 @@ class _QkNormRope(torch.autograd.Function):
         return q_out, k_out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, d_q_out, d_k_out):
         q, k, w_q, w_k, positions, inv_freq = ctx.saved_tensors
         eps, interleaved, heads_first = ctx.how
