@@ -85,8 +85,9 @@ TreePlan tree_plan(const spfa_cache_t* c, const spfa_tree_t* t) {
   const double units = (double)tiles * (double)c->heads * (double)blocks;
   p.workers = units < (double)most ? (int)units : (int)most;
   if (p.workers < 1) p.workers = 1;
-  // (a table of one block cuts no item; the merge has a workgroup per part and row, up to 32)
-  s.merge_rows = blocks <= 1 ? 0 : (int)(rows < 1 ? 1 : rows < 32 ? rows : 32);
+  // (a table of one block cuts no item; the merge has a workgroup per part and row, up to 16: with 32 the many
+  // without a row cost 1 us)
+  s.merge_rows = blocks <= 1 ? 0 : (int)(rows < 1 ? 1 : rows < 16 ? rows : 16);
   p.part_bytes = round256((size_t)p.workers * sizeof(TreePart));
   p.state_bytes = s.merge_rows ? round256((size_t)2 * p.workers * M * sizeof(float)) : 0;
   p.acc_bytes = s.merge_rows ? round256((size_t)2 * p.workers * M * s.dp * sizeof(float)) : 0;

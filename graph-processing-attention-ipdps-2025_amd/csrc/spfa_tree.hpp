@@ -948,7 +948,7 @@ __global__ __launch_bounds__(256, narrow_waves(CODE, DP, NR)) void tree_narrow_k
 // into LDS in the form the products take them (so looking up, decoding and reordering is done once for
 // all rows), then works on its own 32 rows.  One buffer: while a workgroup refills it, the CU's other one
 // computes.  Bound by the softmax's vector instructions (exponentials, packing, maxima): 6 sequences of up
-// to 5000 tokens, 488 rows for each of 8 heads of 64, 55 us and the merge 13 us; over long contexts 430 TFLOP/s.
+// to 5000 tokens, 488 rows for each of 8 heads of 64, 55 us and the merge 9 us; over long contexts 430 TFLOP/s.
 template <int DP>
 struct WideLds {
   static constexpr int kRows = 32 * kTreeWaves;
@@ -1166,93 +1166,71 @@ __global__ __launch_bounds__(256, wide_groups(DP)) void tree_wide_kernel(TreeArg
 }
 
 // Joins the parts of the items that were cut: workgroup (w, y) takes rows of the item whose last part
-// workgroup w of tree_kernel had.  32 lanes hold a row's elements; where an item has many parts, S such
-// groups of the workgroup's eight share a row's parts and meet in LDS, so that few rows do not wait
-// for long chains of loads (a group has kMergeBatch parts on the way at a time).
+// workgroup w had.  DP / 4 lanes hold a row's elements; where an item has many parts, S such groups of the
+// workgroup share a row's parts and meet in LDS, so that few rows do not wait for long chains of loads (a
+// group has kMergeBatch parts on the way at a time).
 constexpr int kMergeBatch = 8;
 // (CODE only keeps the object files' copies apart.)
 template <typename T, int CODE, int DP>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs g, int M) {
-  constexpr int N = DP / 32, V = N < 4 ? N : 4;  // elements per lane, as pieces of V
-  typedef float vec __attribute__((ext_vector_type(V)));
-  __shared__ __align__(16) float acc[8][DP];
-  __shared__ float2 state[8];
+  constexpr int kLanes = DP / 4, kGroups = 256 / kLanes;
+  __shared__ __align__(16) float4v acc[kGroups][kLanes];
+  __shared__ float2 state[kGroups];
   const int w = blockIdx.x;
   const TreePart part = g.part[w];
   if (part.seq < 0) return;
   const TreeSeq sq = tree_seq(g, part.seq, M);
   const int tile0 = part.tile * M, n_rows = sq.n * g.group;
   const int live_rows = n_rows - tile0 < M ? n_rows - tile0 : M;
-  const int grp = threadIdx.x >> 5, c = threadIdx.x & 31;
+  const int grp = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
   const int parts = w - part.first + 1;
-  const int S = parts <= kMergeBatch ? 1 : parts <= 2 * kMergeBatch ? 2 : parts <= 4 * kMergeBatch ? 4 : 8;
-  const int per = 8 / S, sub = grp % S;
+  const int share = parts <= kMergeBatch ? 1 : parts <= 2 * kMergeBatch ? 2 : parts <= 4 * kMergeBatch ? 4 : 8;
+  const int S = share < kGroups ? share : kGroups, per = kGroups / S, sub = grp % S;
   for (int r0 = blockIdx.y * per; r0 < live_rows; r0 += gridDim.y * per) {
     const int r = r0 + grp / S;
-    float m = kNegInf, l = 0.f, x[N] = {};
+    float m = kNegInf, l = 0.f;
+    float4v x = {0.f, 0.f, 0.f, 0.f};
+    auto join = [&](float m2, float l2, const float4v& x2) {
+      const float mn = fmaxf(m, m2);
+      const float a = m == kNegInf ? 1.f : tree_shrink(m - mn);
+      const float b = m2 == kNegInf ? 1.f : tree_shrink(m2 - mn);
+      m = mn;
+      l = l * a + l2 * b;
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = x[e] * a + x2[e] * b;
+    };
     if (r < live_rows) {
       for (int p0 = part.first + sub; p0 <= w; p0 += S * kMergeBatch) {
         float pm[kMergeBatch], pl[kMergeBatch];
-        vec px[kMergeBatch][N / V];
+        float4v px[kMergeBatch];
 #pragma unroll
         for (int u = 0; u < kMergeBatch; u++) {
           const int p = p0 + S * u <= w ? p0 + S * u : w;
           const int64_t at = (p == part.first ? 2 * (int64_t)p + 1 : 2 * (int64_t)p) * M + r;
           pm[u] = g.pm[at];
           pl[u] = g.pl[at];
-#pragma unroll
-          for (int i = 0; i < N / V; i++) px[u][i] = *reinterpret_cast<const vec*>(g.pacc + at * DP + V * (32 * i + c));
+          px[u] = *reinterpret_cast<const float4v*>(g.pacc + at * DP + 4 * c);
         }
 #pragma unroll
-        for (int u = 0; u < kMergeBatch; u++) {
-          if (p0 + S * u > w || pl[u] == 0.f) continue;  // (past the last part, or nothing attended there)
-          const float mn = fmaxf(m, pm[u]);
-          const float a = m == kNegInf ? 1.f : tree_shrink(m - mn);
-          const float b = pm[u] == kNegInf ? 1.f : tree_shrink(pm[u] - mn);
-          m = mn;
-          l = l * a + pl[u] * b;
-#pragma unroll
-          for (int i = 0; i < N / V; i++)
-#pragma unroll
-            for (int e = 0; e < V; e++) x[i * V + e] = x[i * V + e] * a + px[u][i][e] * b;
-        }
+        for (int u = 0; u < kMergeBatch; u++)
+          if (p0 + S * u <= w && pl[u] != 0.f) join(pm[u], pl[u], px[u]);  // (0: nothing attended there)
       }
     }
     if (S > 1) {
       __syncthreads();
       if (c == 0) state[grp] = float2{m, l};
-#pragma unroll
-      for (int i = 0; i < N / V; i++)
-#pragma unroll
-        for (int e = 0; e < V; e++) acc[grp][V * (32 * i + c) + e] = x[i * V + e];
+      acc[grp][c] = x;
       __syncthreads();
-      if (sub == 0) {
-        for (int k = grp + 1; k < grp + S; k++) {
-          const float2 st = state[k];
-          if (st.y == 0.f) continue;
-          const float mn = fmaxf(m, st.x);
-          const float a = m == kNegInf ? 1.f : tree_shrink(m - mn);
-          const float b = st.x == kNegInf ? 1.f : tree_shrink(st.x - mn);
-          m = mn;
-          l = l * a + st.y * b;
-#pragma unroll
-          for (int i = 0; i < N / V; i++)
-#pragma unroll
-            for (int e = 0; e < V; e++) x[i * V + e] = x[i * V + e] * a + acc[k][V * (32 * i + c) + e] * b;
-        }
-      }
+      if (sub == 0)
+        for (int k = grp + 1; k < grp + S; k++)
+          if (state[k].y != 0.f) join(state[k].x, state[k].y, acc[k][c]);
     }
     if (sub == 0 && r < live_rows) {
       const int rr = tile0 + r;
       const int nd = (int)fast_div((uint32_t)rr, g.group_magic, g.group_shift), gi = rr - nd * g.group;
       const TreeWeights tw = tree_weights(g, sq.row0 + nd, part.head * g.group + gi, m, l);
-#pragma unroll
-      for (int i = 0; i < N / V; i++) {
-        float y[V];
-#pragma unroll
-        for (int e = 0; e < V; e++) y[e] = x[i * V + e];
-        tree_store<T, V>(g, sq.row0 + nd, part.head * g.group + gi, V * (32 * i + c), tw, y);
-      }
+      const float y[4] = {x[0], x[1], x[2], x[3]};
+      tree_store<T, 4>(g, sq.row0 + nd, part.head * g.group + gi, 4 * c, tw, y);
       if (c == 0) tree_store_state(g, sq.row0 + nd, part.head * g.group + gi, tw);
     }
   }
