@@ -1013,3 +1013,44 @@ def test_replays_from_a_graph():
         torch.cuda.synchronize()
         for a, b in zip(got, (*results, kc, vc, ks, vs)):
             assert torch.equal(a, b), rep
+
+
+@pytest.mark.parametrize("dt,code,d", [(F16, "none", 64), (BF16, "int8", 128)])
+def test_many_rows_replay_with_other_lengths(dt, code, d):
+    """The kernel of many rows, captured and replayed while the contexts change, beside eager calls on
+    another stream."""
+    r = Run(31, dt, code, d, 16, 2, 8, True, [700, 90, 0], [60, 40, 9], "tree", **ROOM)
+    out = torch.empty(r.q.shape, dtype=dt, device=DEV)
+    r.call(out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r.call(out)
+    side = torch.cuda.Stream()
+    for ctx in ([700, 90, 0], [10, 89, 0], [333, 0, 0]):  # (fewer cached tokens: nodes are read from other places)
+        r.ctx_t.copy_(torch.tensor(ctx, dtype=torch.int32))
+        torch.cuda.synchronize()
+        want = torch.empty_like(out)
+        with torch.cuda.stream(side):
+            r.call(want)
+        out.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        r.ctx = ctx
+        full = type(r).read
+        r.read = lambda i: [x[:r.ctx[i] + r.nodes[i]] for x in full(r, i)]
+        r.check(out)
+
+
+def test_cache_of_more_slots_than_31_bits():
+    """Slot numbers past 2^31 (pages that are all the same memory, for reading)."""
+    m = _mod("spfa_cache")
+    one = [torch.randn(1, 16, 2, 8, generator=_gen(i), device=DEV).to(BF16) for i in (1, 2)]
+    kc, vc = [x.expand((1 << 28) + 5, 16, 2, 8) for x in one]
+    slots = torch.tensor([0, 5, (1 << 31) - 1, (1 << 31) + 7, (1 << 32) + 79, (1 << 32) + 80, -1, 1 << 40], device=DEV)
+    ko, vo = [torch.full((8, 2, 8), 3.0, dtype=BF16, device=DEV) for _ in range(2)]
+    m.read(kc, vc, slots, ko, vo)
+    for x, y in zip(one, (ko, vo)):
+        assert torch.equal(y[:5], x[0, (slots[:5] % 16)])
+        assert (y[5:] == 3.0).all()
