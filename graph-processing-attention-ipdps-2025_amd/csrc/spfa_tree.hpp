@@ -261,7 +261,12 @@ struct TreeTypes {
   static constexpr int VW = VB / 4;
   static constexpr int QF = DP / 32;           // pieces of a query
   using Tv = std::conditional_t<kCoded, bf16, T>;  // (8-bit values times any scale need bf16's range)
-  static constexpr bool kTwoParts = kCoded && __is_same(T, f16);  // weights of f16 calls in two bf16 parts
+  // Weights in two bf16 parts: needed where f16 calls meet 8-bit codes (one part has 8 of their 11 bits),
+  // and with bf16 calls what keeps the result to its own rounding (one part adds as much again).  The
+  // narrow kernel has room and time for it (2 x 200001 bf16 tokens 225 -> 226 us, 64 x 8191 e4m3 131 -> 132);
+  // the wide one's registers spill with bf16 heads of 128.
+  static constexpr bool kTwoNarrow = kCoded || __is_same(T, bf16);
+  static constexpr bool kTwoWide = kCoded && __is_same(T, f16);
 };
 
 // This workgroup's run of the line of all items' blocks, item by item.
@@ -654,7 +659,7 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t x) {
 }
 
 // The softmax state of 16 rows and what a tile of 32 keys does to it.
-template <typename T, int CODE, int DP>
+template <typename T, int CODE, int DP, bool TWO>
 struct TreeState {
   using Ty = TreeTypes<T, CODE, DP>;
   using Tv = typename Ty::Tv;
@@ -722,14 +727,14 @@ struct TreeState {
       }
       const uint32_t hi = tree_pack<Tv>(p[0], p[1]);
       pf[x] = hi;
-      if constexpr (Ty::kTwoParts)
+      if constexpr (TWO)
         pl[x] = tree_pack<Tv>(p[0] - __builtin_bit_cast(float, hi << 16), p[1] - __builtin_bit_cast(float, hi & 0xffff0000u));
     }
     l += sum;
   }
   __device__ __forceinline__ void add(const uint4v& f, int e) {
     o[e] = tree_mfma<Tv>(f, pf, o[e]);
-    if constexpr (Ty::kTwoParts) o[e] = tree_mfma<Tv>(f, pl, o[e]);
+    if constexpr (TWO) o[e] = tree_mfma<Tv>(f, pl, o[e]);
   }
   // Adds the infinities and NaN among the values, and only those, to the rows that attend their keys:
   // how many of each sign a row has comes from products of ones.
@@ -865,7 +870,7 @@ __global__ __launch_bounds__(256, narrow_waves(CODE, DP, NR)) void tree_narrow_k
     int t = it.blk0 * 4 + wave;
     TreeKeys<T, CODE, DP, ROWS> keys;
     TreeQueries<T, CODE, DP, ROWS> q[NR];
-    TreeState<T, CODE, DP> st[NR];
+    TreeState<T, CODE, DP, Ty::kTwoNarrow> st[NR];
     keys.start(a, it, t_end, reinterpret_cast<int64_t*>(mine));
 #pragma unroll
     for (int n = 0; n < NR; n++) st[n].start();
@@ -987,7 +992,7 @@ __global__ __launch_bounds__(256, wide_groups(DP)) void tree_wide_kernel(TreeArg
     int t = it.blk0 * 4;  // first tile of the block
     TreeKeys<T, CODE, DP, ROWS> keys;
     TreeQueries<T, CODE, DP, ROWS> q[NR];
-    TreeState<T, CODE, DP> st[NR];
+    TreeState<T, CODE, DP, Ty::kTwoWide> st[NR];
     keys.start(a, it, t_end, reinterpret_cast<int64_t*>(mine));
 #pragma unroll
     for (int n = 0; n < NR; n++) st[n].start();
