@@ -247,7 +247,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs g) {
 #pragma unroll
           for (int e = 0; e < E; e++) ss = __builtin_fmaf(xa[j][e], xa[j][e], __builtin_fmaf(xb[j][e], xb[j][e], ss));
         }
-        const float r = 1.f / sqrtf(group_sum<LPV>(ss) / (float)g.d + g.eps);
+        // (with eps = 0 lanes without a vector would add 0 * infinity to the weights' sums)
+        const float sq = group_sum<LPV>(ss) / (float)g.d + g.eps, r = ok ? 1.f / sqrtf(sq) : 0.f;
         if constexpr (!GRAD) {
           if (ok) {
 #pragma unroll
