@@ -664,6 +664,10 @@ struct TreeState {
   using Ty = TreeTypes<T, CODE, DP>;
   using Tv = typename Ty::Tv;
   static constexpr int EB = Ty::EB;
+  // The reference is taken this much below the largest score.  f16 weights are subnormal below 2^-14 and
+  // zero below 2^-25: with 2^7 for the largest one (and 2^15 where the slack is used up, f16 ends at 2^16)
+  // a weight keeps its 11 bits down to 2^-21 of it, and is off by 2^-32 of it at most below that.
+  static constexpr float kLift = __is_same(Tv, f16) ? 7.f : 0.f;
   f32x4t o[EB];       // element EB * (4 g + v) + e of row c, unnormalised, against ref
   float ref, top, l;  // reference of the scores (log2 units), this lane's largest and its sum of weights
   uint4v pf, pl;
@@ -704,8 +708,8 @@ struct TreeState {
     // (the largest of this lane's keys; the row's four lanes only meet when one of them calls for it)
     if constexpr (!Ty::kCoded) mx *= scale;
     top = fmaxf(top, mx);
-    if (__builtin_amdgcn_ballot_w64(mx > ref + kTreeSlack) != 0) {
-      const float now = fmaxf(ref, row_max(mx));
+    if (__builtin_amdgcn_ballot_w64(mx > ref + (kTreeSlack + kLift)) != 0) {
+      const float now = fmaxf(ref, row_max(mx) - kLift);
       const float alpha = tree_shrink(ref - now);
       ref = now;
       l *= alpha;

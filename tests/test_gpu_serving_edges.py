@@ -1,12 +1,15 @@
 """Inputs at the edges of what the operators around masked attention take, on the GPU against the
 float64 oracle: the cases, tolerances' units and helpers are those of test_gpu_serving.py."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
 from helpers import np64
 from oracle import serve_oracle as sv
-from test_gpu_serving import BF16, DEV, F16, F32, HALF, TINY, U, _close, _gen, _mod, _ones, _pair_size, _rope_inputs
+from test_gpu_serving import (BF16, DEV, F16, F32, HALF, TINY, U, Run, _close, _gen, _mod, _ones, _pair_size,
+                              _rope_inputs)
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +44,39 @@ def test_rope_gradients_without_eps(case):
         gx, gw, sx, sw = sv.norm_rope_backward(np64(x), _ones(ww, d), p, fr, 0.0, inter, np64(dy))
         _close(dx, gx, HALF[dt] * np.abs(gx) + TINY[dt] + (d + 60) * U * sx, "gradient")
         _close(dww, gw, (d + 60 + tokens * heads) * U * sw + TINY[F32], "weights' gradient")
+
+
+# ------------------------------------------------------------------------------------------------
+# tree attention
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("far", [14.25, 17.46875])
+@pytest.mark.parametrize("nodes", [1, 20, 90])
+def test_tree_one_key_far_above_many(nodes, far):
+    """f16 weights: one key whose score is `far` (20.6 or 25.2 powers of two) above those of all the others,
+    which still show in the result.
+
+    What the other weights lose: they are f16 numbers next to a largest one of at least 2^7, each off by at
+    most half of f16's smallest step, 2^-25, where that is more than 2^-11 of it: 2^-32 of the sum a key."""
+    d, hk, n, seqs = 64, 8, 1500, 64  # (so many that a workgroup has all keys of an item)
+    r = Run(41, F16, "none", d, 64, hk, 1, True, [n - nodes] * seqs, [nodes] * seqs, "chain", strided=False)
+    kc, vc, _, _ = r.cache
+    k = torch.zeros(seqs, n, hk, d, device=DEV)
+    k[:, 1:, :, 0] = -far / 2  # exact in f16, and so are the scores: -16 * far / 2 / 8
+    v = 64 * (1 + 0.25 * torch.rand(seqs, n, hk, d, generator=_gen(42), device=DEV))
+    v[:, 0] = 0
+    k, v = k.to(F16), v.to(F16)
+    _mod("spfa_cache").write(k.flatten(0, 1), v.flatten(0, 1), torch.cat(r.slots), kc, vc)
+    r.q = torch.zeros(seqs * nodes, hk, d, dtype=F16, device=DEV)
+    r.q[..., 0] = 16
+    out = torch.empty(r.q.shape, dtype=F16, device=DEV)
+    r.call(out)
+    for s in (0, 33, seqs - 1):
+        for h in (0, hk - 1):
+            for i in sorted({0, nodes // 2, nodes - 1}):
+                live = n - nodes + i + 1
+                row = s * nodes + i
+                o, _, _, a, s_abs = sv.tree_attention(np64(r.q[row:row + 1, h]), np64(k[s, :live, h]), np64(v[s, :live, h]),
+                                                      np.ones((1, live), dtype=bool), 1 / math.sqrt(d))
+                rel = HALF[F16] + (2 * n + 40) * U + 4 * (d + 8) * U * s_abs[0]
+                _close(out[row, h], o[0], HALF[F16] * np.abs(o[0]) + a[0] * rel + live * 2.0 ** -32 * 80 + TINY[F16],
+                       "sequence %d head %d row %d" % (s, h, i))
