@@ -768,19 +768,24 @@ struct TreeState {
     }
   }
   // The rows' results into LDS: state (max, sum) and unnormalised elements, `stride` floats a row.
-  // (odd: the elements' places hold sums that are added)
-  __device__ __forceinline__ void leave(float* acc, float2* state, int row, int stride, bool odd) const {
+  // (odd: the elements' places hold sums that are added)  False if an element of the lane is not finite.
+  __device__ __forceinline__ bool leave(float* acc, float2* state, int row, int stride, bool odd) const {
     const int c = lane_id() & 15, g = lane_id() >> 4;
     const float most = row_max(top);
     const float f = most == kNegInf ? 1.f : __builtin_amdgcn_exp2f(ref - most);
     const float lt = row_sum(l) * f;
     if (g == 0) state[row + c] = float2{most, lt};
+    float z = 0.f;
 #pragma unroll
     for (int v = 0; v < 4; v++) {
       float* to = acc + (row + c) * stride + EB * (4 * g + v);
 #pragma unroll
-      for (int e = 0; e < EB; e++) to[e] = odd ? o[e][v] * f + to[e] : o[e][v] * f;
+      for (int e = 0; e < EB; e++) {
+        z = __builtin_fmaf(o[e][v], 0.f, z);
+        to[e] = odd ? o[e][v] * f + to[e] : o[e][v] * f;
+      }
     }
+    return z == 0.f;
   }
 };
 
@@ -869,6 +874,10 @@ __global__ __launch_bounds__(256, narrow_waves(CODE, DP, NR)) void tree_narrow_k
   if (threadIdx.x == 0) a.part[it.w].seq = -1;
   if (!any) return;
   const float scale = __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, a.scale_log2)));
+  // Tiles that every row attends are not looked through for infinities and NaN among the values.  Such a
+  // value shows in the results (as NaN, times a weight that is zero or whose second part is not above zero),
+  // and the wavefront works on its tiles once more, now screening all of them.
+  bool screened = false;
   while (it.item(a, M)) {
     const int t_all = (it.sq.len + 31) / 32, t_end = it.blk1 * 4 < t_all ? it.blk1 * 4 : t_all;
     int t = it.blk0 * 4 + wave;
@@ -898,7 +907,7 @@ __global__ __launch_bounds__(256, narrow_waves(CODE, DP, NR)) void tree_narrow_k
 #pragma unroll
       for (int n = 0; n < NR; n++) q[n].flip(a.flip);
     }
-    const int t_full = it.sq.ctx / 32;  // tiles below lie before the tree
+    const int t_full = screened ? 0 : it.sq.ctx / 32;  // tiles below lie before the tree
     for (; t < t_end; t += kTreeWaves) {
       const uint32_t exist = exist_next;
       const bool whole = exist == 0xffffffffu && t < t_full;  // every row attends all 32 keys
@@ -943,8 +952,14 @@ __global__ __launch_bounds__(256, narrow_waves(CODE, DP, NR)) void tree_narrow_k
       }
       keys.load_v(a.d);
     }
+    bool fine = true;
 #pragma unroll
-    for (int n = 0; n < NR; n++) st[n].leave(acc_lds, state_lds, wave * M + 16 * n, Lds::kStride, odd);
+    for (int n = 0; n < NR; n++) fine &= st[n].leave(acc_lds, state_lds, wave * M + 16 * n, Lds::kStride, odd);
+    if (__builtin_expect(!screened && __builtin_amdgcn_ballot_w64(!fine) != 0, 0)) {
+      screened = true;
+      continue;  // (the same item)
+    }
+    screened = false;
     __syncthreads();
     tree_join<T, DP>(a, it, acc_lds, state_lds, kTreeWaves, M);
     __syncthreads();  // (all of it has been read: the next item may use the LDS)
@@ -966,7 +981,7 @@ struct WideLds {
   static constexpr int kJoin = kRows * kStride * 4;
   static constexpr int kShared = kTreeWaves * kFrags * 1024 > kJoin ? kTreeWaves * kFrags * 1024 : kJoin;
   static constexpr int kState = kRows * 8;
-  static constexpr int kTile = 64 * 8 + 2 * 32 * 4 + 16;  // places, scales, existing keys and whether there are odd values
+  static constexpr int kTile = 64 * 8 + 2 * 32 * 4 + 16;  // places, scales, existing keys, whether values and results are odd
   static constexpr int kBytes = kShared + kState + kTreeWaves * kTile;
 };
 constexpr int wide_groups(int dp) { return dp == 256 ? 1 : 2; }  // workgroups per CU
@@ -991,6 +1006,7 @@ __global__ __launch_bounds__(256, wide_groups(DP)) void tree_wide_kernel(TreeArg
   if (threadIdx.x == 0) a.part[it.w].seq = -1;
   if (!any) return;
   const float scale = __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, a.scale_log2)));
+  bool screened = false;  // (as in the narrow kernel, the whole workgroup together)
   while (it.item(a, M)) {
     const int t_all = (it.sq.len + 31) / 32, t_end = it.blk1 * 4 < t_all ? it.blk1 * 4 : t_all;
     int t = it.blk0 * 4;  // first tile of the block
@@ -1016,7 +1032,7 @@ __global__ __launch_bounds__(256, wide_groups(DP)) void tree_wide_kernel(TreeArg
 #pragma unroll
       for (int n = 0; n < NR; n++) q[n].flip(a.flip);
     }
-    const int t_full = it.sq.ctx / 32;  // tiles below lie before the tree
+    const int t_full = screened ? 0 : it.sq.ctx / 32;  // tiles below lie before the tree
     for (; t < t_end; t += kTreeWaves) {
       // ---- this wavefront's tile into LDS ----
       const int tt = t + wave;
@@ -1164,9 +1180,16 @@ __global__ __launch_bounds__(256, wide_groups(DP)) void tree_wide_kernel(TreeArg
       }
       __syncthreads();
     }
+    bool fine = true;
 #pragma unroll
-    for (int n = 0; n < NR; n++) st[n].leave(acc_lds, state_lds, 16 * (wave * NR + n), Lds::kStride, false);
+    for (int n = 0; n < NR; n++) fine &= st[n].leave(acc_lds, state_lds, 16 * (wave * NR + n), Lds::kStride, false);
+    word_mine[2] = __builtin_amdgcn_ballot_w64(!fine) != 0;
     __syncthreads();
+    uint32_t bad = 0;
+#pragma unroll
+    for (int j = 0; j < kTreeWaves; j++) bad |= reinterpret_cast<const uint32_t*>(tiles + j * Lds::kTile + 64 * 8 + 2 * 32 * 4)[2];
+    screened = !screened && uniform((int)bad) != 0;
+    if (screened) continue;
     tree_join<T, DP>(a, it, acc_lds, state_lds, 1, M);
     __syncthreads();  // (all of it has been read: the next item may use the LDS)
     if (threadIdx.x == 0) it.name_part(a);

@@ -443,7 +443,8 @@ int spfa_cache_read(const spfa_cache_t* c, const void* slots, int slot_bytes, in
  * The arrays on the device are held to the sizes given here: a position whose page entry is not in
  * [0, pages) or lies past page_table is masked, a negative ctx_len counts as 0, offsets are cut to
  * [0, rows], nodes past 64 * mask_words have no bits.  What masked places hold (NaN included) does
- * not reach a row that masks them. */
+ * not reach a row that masks them; an infinity among the values reaches the rows that attend it as
+ * the formula has it, however small its weight. */
 typedef struct spfa_tree {
   const void* q;                  /* [rows, heads_q, d], unit stride along d */
   void* out;                      /* likewise */

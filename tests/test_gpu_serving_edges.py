@@ -8,7 +8,7 @@ import torch
 
 from helpers import np64
 from oracle import serve_oracle as sv
-from test_gpu_serving import (BF16, DEV, F16, F32, HALF, TINY, U, Run, _close, _gen, _mod, _ones, _pair_size,
+from test_gpu_serving import (BF16, DEV, F16, F32, HALF, ROOM, TINY, U, Run, _close, _gen, _mod, _ones, _pair_size,
                               _rope_inputs)
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +80,45 @@ def test_tree_one_key_far_above_many(nodes, far):
                 rel = HALF[F16] + (2 * n + 40) * U + 4 * (d + 8) * U * s_abs[0]
                 _close(out[row, h], o[0], HALF[F16] * np.abs(o[0]) + a[0] * rel + live * 2.0 ** -32 * 80 + TINY[F16],
                        "sequence %d head %d row %d" % (s, h, i))
+
+
+@pytest.mark.parametrize("dt,code", [(BF16, "none"), (F16, "none"), (BF16, "e4m3"), (F16, "e4m3"), (BF16, "int8"), (F16, "int8")])
+@pytest.mark.parametrize("d,nodes", [(64, 1), (64, 20), (128, 1), (128, 40), (256, 9), (64, 250), (128, 250), (256, 250)])
+def test_tree_infinities_in_front_of_the_tree(dt, code, d, nodes):
+    """Cached tokens that every row attends hold infinities and NaN, some where weights are tiny."""
+    r = Run(43, dt, code, d, 16, 1, 2, True, [700, 140, 9], [nodes, 4, 3], "random", **(ROOM if nodes > 100 else {}))
+    kc, vc, ks, vs = r.cache
+    sick = {0: [7, 200, 699], 1: [40], 2: []}
+    for i in sick:
+        for j in sick[i]:
+            slot = int(r.slots[i][j])
+            p, at = slot // 16, slot % 16
+            if code == "none":
+                vc[p, at, 0, 5] = float("inf")
+                vc[p, at, 0, d - 3] = float("-inf")
+                vc[p, at, 0, 9] = float("nan") if j == 200 else float("inf") if j == 7 else 0.0
+            elif code == "e4m3" and j != 200:
+                vc[p, at, 0].view(torch.uint8)[7] = 0x7f
+            else:
+                vs[p, at, 0] = float("inf")
+    if code == "none":  # the keys of one of them: scores far below the others'
+        slot = int(r.slots[0][7])
+        kc[slot // 16, slot % 16, 0] = (-4 * r.q[r.off[0], 0].float()).to(dt)
+    out = torch.empty(r.q.shape, dtype=dt, device=DEV)
+    r.call(out)
+    o, q = np64(out), np64(r.q)
+    for i in range(3):
+        kk, vv = r.read(i)
+        lv = r.live(i)
+        for hq in range(2):
+            rows = np.arange(r.off[i], r.off[i + 1])
+            with np.errstate(all="ignore"):
+                want, _, _, a, s_abs = sv.tree_attention(q[rows, hq], kk[:, 0], vv[:, 0], lv, 1 / math.sqrt(d))
+            for n, row in enumerate(rows):
+                w, g = want[n], o[row, hq]
+                fine = np.isfinite(w)
+                assert np.array_equal(g[~fine], w[~fine], equal_nan=True), (i, n, hq)
+                eps_p = 2.0 ** -16 if (code != "none" and dt == F16) else HALF[dt]
+                rel = eps_p + (2 * lv.shape[1] + 40) * U + 4 * (d + 8) * U * s_abs[n]
+                tol = HALF[dt] * np.abs(w[fine]) + a[n][fine] * rel * (1 + HALF[dt]) + TINY[dt]
+                assert (np.abs(g[fine] - w[fine]) <= tol).all(), (i, n, hq)
