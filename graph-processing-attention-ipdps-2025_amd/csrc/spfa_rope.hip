@@ -445,8 +445,9 @@ int rope_check(const spfa_rope_t* p) {
   if (p->heads_q > (1 << 20) || p->heads_k > (1 << 20)) return SPFA_ERR_BAD_ARG;
   if (p->rot < 0 || p->rot > p->d || p->rot % 2) return SPFA_ERR_BAD_ARG;
   if (p->position_bytes != 4 && p->position_bytes != 8) return SPFA_ERR_BAD_ARG;
-  if (p->batch > 0 && p->tokens > INT64_MAX / 2048 / (p->batch * ((p->heads_q > p->heads_k ? p->heads_q : p->heads_k) + 1)))
-    return SPFA_ERR_BAD_ARG;
+  // (the vectors' number, and that times 2048, fit 64 bits; no product here leaves them)
+  const int64_t most = INT64_MAX / 2048 / ((p->heads_q > p->heads_k ? p->heads_q : p->heads_k) + 1);
+  if (p->batch > most || (p->batch > 0 && p->tokens > most / p->batch)) return SPFA_ERR_BAD_ARG;
   return SPFA_OK;
 }
 
