@@ -26,6 +26,14 @@ inline spfa_heads_t heads_of(const torch::Tensor& t) {
   return spfa_heads_t{t.data_ptr(), n == 4 ? stride_of(t, 0) : 0, stride_of(t, n - 3), stride_of(t, n - 2)};
 }
 
+// The very same elements in the same places (the stride of a dimension of one element is nobody's).
+inline bool same_place(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.sizes() != b.sizes() || a.scalar_type() != b.scalar_type()) return false;
+  for (int64_t i = 0; i < a.dim(); i++)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
 // An output overlaps neither itself nor other tensors of the call, except that it may be the very tensor
 // it is computed from row by row (`own`).
 inline void check_output(const torch::Tensor& out, const char* name, std::initializer_list<torch::Tensor> others,
@@ -38,8 +46,8 @@ inline void check_output(const torch::Tensor& out, const char* name, std::initia
                 name, " overlaps another tensor of the call");
   }
   for (const torch::Tensor& x : own)
-    TORCH_CHECK(at::get_overlap_status(out, x) != at::MemOverlapStatus::Partial &&
-                    (out.numel() == 0 || out.data_ptr() != x.data_ptr() || out.strides() == x.strides()),
+    TORCH_CHECK(out.numel() == 0 || same_place(out, x) ||
+                    (at::get_overlap_status(out, x) != at::MemOverlapStatus::Partial && out.data_ptr() != x.data_ptr()),
                 name, " partly overlaps another tensor of the call");
 }
 

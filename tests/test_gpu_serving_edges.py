@@ -46,6 +46,19 @@ def test_rope_gradients_without_eps(case):
         _close(dww, gw, (d + 60 + tokens * heads) * U * sw + TINY[F32], "weights' gradient")
 
 
+def test_rope_in_place_of_one_token_by_another_view():
+    """The stride of a dimension of one is nobody's: the same place stays the same place."""
+    m = _mod("spfa_rope")
+    x = torch.randn(3, 6, 64, generator=_gen(24), device=DEV).to(BF16)[1:2]
+    q, k = x[:, :4], x[:, 4:]
+    pos, f = torch.tensor([5], device=DEV), 100.0 ** (-torch.arange(32, device=DEV, dtype=F32) / 32)
+    want = m.forward(q, k, None, None, pos, f, torch.empty_like(q), torch.empty_like(k))
+    other = [y[0].unsqueeze(0) for y in (q, k)]
+    assert other[0].data_ptr() == q.data_ptr() and other[0].stride() != q.stride()
+    m.forward(q, k, None, None, pos, f, *other)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
 # ------------------------------------------------------------------------------------------------
 # tree attention
 # ------------------------------------------------------------------------------------------------
