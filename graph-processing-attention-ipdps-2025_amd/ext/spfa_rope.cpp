@@ -14,7 +14,7 @@ spfa_rope_t make_rope(const torch::Tensor& q, const torch::Tensor& k, const OptT
                       const torch::Tensor& positions, const torch::Tensor& inv_freq, double eps, bool interleaved) {
   CHECK_ROWS(q);
   CHECK_ROWS(k);
-  CHECK_INPUT(positions);
+  CHECK_ROWS(positions);
   CHECK_INPUT(inv_freq);
   const int64_t n = q.dim();
   TORCH_CHECK((n == 3 || n == 4) && k.dim() == n, "q and k must both be [tokens, heads, d] or [batch, tokens, heads, d]");
@@ -55,11 +55,11 @@ spfa_rope_t make_rope(const torch::Tensor& q, const torch::Tensor& k, const OptT
   p.w_k = w_k.has_value() ? w_k->data_ptr() : nullptr;
   p.position_bytes = spfa_ext::signed_index_bytes(positions, "positions");
   if (positions.dim() == 1) {
-    TORCH_CHECK(positions.size(0) == p.tokens, "positions must be [tokens] or [batch, tokens]");
+    TORCH_CHECK(positions.size(0) == p.tokens, "positions must be [tokens], [1, tokens] or [batch, tokens]");
   } else {
-    TORCH_CHECK(n == 4 && positions.dim() == 2 && positions.size(0) == p.batch && positions.size(1) == p.tokens,
-                "positions must be [tokens] or [batch, tokens]");
-    p.position_stride = p.tokens;
+    TORCH_CHECK(n == 4 && positions.dim() == 2 && (positions.size(0) == p.batch || positions.size(0) == 1) && positions.size(1) == p.tokens,
+                "positions must be [tokens], [1, tokens] or [batch, tokens]");
+    p.position_stride = spfa_ext::stride_of(positions, 0);
   }
   p.positions = positions.data_ptr();
   return p;

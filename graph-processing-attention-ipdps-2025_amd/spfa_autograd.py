@@ -147,7 +147,7 @@ def qk_norm_rope(q, k, w_q, w_k, positions, inv_freq, eps=1e-6, interleaved=Fals
     w_q and w_k.
 
     q, k: [tokens, heads, d] or [batch, tokens, heads, d], any strides outside the last dimension (the
-    slices of a fused projection are fine); w_q, w_k: [d] or None; positions: [tokens] or
-    [batch, tokens] integers; inv_freq: float32 [pairs].  Returns (q, k) as attention() takes them,
+    slices of a fused projection are fine); w_q, w_k: [d] or None; positions: [tokens],
+    [1, tokens] or [batch, tokens] integers; inv_freq: float32 [pairs].  Returns (q, k) as attention() takes them,
     [..., heads, tokens, d], or in the order of the inputs with heads_first=False."""
     return _QkNormRope.apply(q, k, w_q, w_k, positions, inv_freq, eps, interleaved, heads_first)

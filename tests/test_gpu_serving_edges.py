@@ -59,6 +59,28 @@ def test_rope_in_place_of_one_token_by_another_view():
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
 
 
+def test_rope_positions_that_are_broadcast():
+    """One row of positions for all of a batch, as [1, tokens] or expanded, and rows of a wider table."""
+    m = _mod("spfa_rope")
+    case = (BF16, 7, 2, 1, 64, 64, False, BF16, True, False)
+    q, k, w, pos, f = _rope_inputs(case, 23, batch=4)
+    new = lambda: [torch.empty(x.shape, dtype=BF16, device=DEV) for x in (q, k)]
+    for dt in (torch.int32, torch.int64):
+        row = pos[2].to(dt)
+        want = m.forward(q, k, *w, row, f, *new())
+        table = torch.full((4, 20), 99, dtype=dt, device=DEV)
+        table[:, 3:10] = row
+        for p in (row.view(1, 7), row.expand(4, 7), row.repeat(4, 1), table[:, 3:10], table[:1, 3:10]):
+            got = m.forward(q, k, *w, p, f, *new())
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    one = [x[:1] for x in (q, k)]
+    got = m.forward(*one, *w, pos[2].view(1, 7), f, *[torch.empty(x.shape, dtype=BF16, device=DEV) for x in one])
+    assert torch.equal(got[0][0], want[0][0])
+    for p in (pos[:2], pos[:3].contiguous(), pos.t().contiguous().t(), pos[..., None], pos[:, :6]):
+        with pytest.raises((RuntimeError, ValueError)):
+            m.forward(q, k, *w, p, f, *new())
+
+
 # ------------------------------------------------------------------------------------------------
 # tree attention
 # ------------------------------------------------------------------------------------------------
