@@ -82,8 +82,8 @@ std::tuple<torch::Tensor, torch::Tensor> spfa_rope_forward_py(torch::Tensor q, t
   const spfa_rope_t p = make_rope(q, k, w_q, w_k, positions, inv_freq, eps, interleaved);
   check_like(q_out, q, "q_out");
   check_like(k_out, k, "k_out");
-  spfa_ext::check_output(q_out, "q_out", {k, k_out, positions, inv_freq}, {q});
-  spfa_ext::check_output(k_out, "k_out", {q, positions, inv_freq}, {k});
+  spfa_ext::check_output(q_out, "q_out", {k, k_out, w_q, w_k, positions, inv_freq}, {q});
+  spfa_ext::check_output(k_out, "k_out", {q, w_q, w_k, positions, inv_freq}, {k});
   c10::DeviceGuard guard(q.device());
   const spfa_heads_t qo = spfa_ext::heads_of(q_out), ko = spfa_ext::heads_of(k_out);
   spfa_ext::raise_on_error(spfa_qk_norm_rope_forward(&p, &qo, &ko, spfa_ext::current_stream(q)));
@@ -101,8 +101,8 @@ std::tuple<torch::Tensor, torch::Tensor> spfa_rope_backward_py(torch::Tensor q, 
   check_like(d_k_out, k, "d_k_out");
   check_like(d_q, q, "d_q");
   check_like(d_k, k, "d_k");
-  spfa_ext::check_output(d_q, "d_q", {k, d_k_out, d_k, positions, inv_freq}, {q, d_q_out});
-  spfa_ext::check_output(d_k, "d_k", {q, d_q_out, positions, inv_freq}, {k, d_k_out});
+  spfa_ext::check_output(d_q, "d_q", {k, d_k_out, d_k, w_q, w_k, positions, inv_freq}, {q, d_q_out});
+  spfa_ext::check_output(d_k, "d_k", {q, d_q_out, w_q, w_k, positions, inv_freq}, {k, d_k_out});
   for (const OptTensor* w : {&d_w_q, &d_w_k}) {
     if (!w->has_value()) continue;
     const torch::Tensor& t = **w;
@@ -110,7 +110,9 @@ std::tuple<torch::Tensor, torch::Tensor> spfa_rope_backward_py(torch::Tensor q, 
     CHECK_SAME_DEVICE(t, q);
     TORCH_CHECK(t.dim() == 1 && t.size(0) == p.d && t.scalar_type() == torch::kFloat32, "d_w_q and d_w_k must be float32 [d]");
   }
-  if (d_w_q.has_value() && d_w_k.has_value()) spfa_ext::check_output(*d_w_q, "d_w_q", {*d_w_k});
+  // (in place of its own weights: these have been read when the sums are written)
+  if (d_w_q.has_value()) spfa_ext::check_output(*d_w_q, "d_w_q", {q, k, w_k, positions, inv_freq, d_q_out, d_k_out, d_q, d_k, d_w_k}, {w_q});
+  if (d_w_k.has_value()) spfa_ext::check_output(*d_w_k, "d_w_k", {q, k, w_q, positions, inv_freq, d_q_out, d_k_out, d_q, d_k}, {w_k});
   c10::DeviceGuard guard(q.device());
   const spfa_heads_t dqo = spfa_ext::heads_of(d_q_out), dko = spfa_ext::heads_of(d_k_out);
   const spfa_heads_t dq = spfa_ext::heads_of(d_q), dk = spfa_ext::heads_of(d_k);

@@ -34,21 +34,27 @@ inline bool same_place(const torch::Tensor& a, const torch::Tensor& b) {
   return true;
 }
 
-// An output overlaps neither itself nor other tensors of the call, except that it may be the very tensor
-// it is computed from row by row (`own`).
-inline void check_output(const torch::Tensor& out, const char* name, std::initializer_list<torch::Tensor> others,
-                         std::initializer_list<torch::Tensor> own = {}) {
+// An output overlaps neither itself nor other tensors of the call (those that are not there aside), except
+// that it may be the very tensor it is computed from row by row (`own`).  Of tensors with gaps only those
+// that begin at the same place are known to overlap: slices of one buffer may lie in each other's gaps.
+inline void check_output(const torch::Tensor& out, const char* name, std::initializer_list<OptTensor> others,
+                         std::initializer_list<OptTensor> own = {}) {
   TORCH_CHECK(at::has_internal_overlap(out) != at::MemOverlap::Yes, name, " must not overlap itself");
-  for (const torch::Tensor& x : others) {
+  for (const OptTensor& t : others) {
+    if (!t.has_value()) continue;
+    const torch::Tensor& x = *t;
     const auto o = at::get_overlap_status(out, x);
     TORCH_CHECK(o != at::MemOverlapStatus::Partial && o != at::MemOverlapStatus::Full &&
                     (out.numel() == 0 || x.numel() == 0 || out.data_ptr() != x.data_ptr()),
                 name, " overlaps another tensor of the call");
   }
-  for (const torch::Tensor& x : own)
+  for (const OptTensor& t : own) {
+    if (!t.has_value()) continue;
+    const torch::Tensor& x = *t;
     TORCH_CHECK(out.numel() == 0 || same_place(out, x) ||
                     (at::get_overlap_status(out, x) != at::MemOverlapStatus::Partial && out.data_ptr() != x.data_ptr()),
                 name, " partly overlaps another tensor of the call");
+  }
 }
 
 inline int32_t serve_dtype(const torch::Tensor& t, const char* name) {

@@ -81,6 +81,37 @@ def test_rope_positions_that_are_broadcast():
             m.forward(q, k, *w, p, f, *new())
 
 
+def test_rope_outputs_over_weights_positions_and_each_other_are_refused():
+    m = _mod("spfa_rope")
+    q, k = [torch.randn(4, h, 64, generator=_gen(h), device=DEV) for h in (2, 1)]
+    w = [torch.ones(64, device=DEV) for _ in range(2)]
+    pos, f = torch.arange(64, device=DEV)[:4], torch.ones(32, device=DEV)
+    new = lambda: [torch.empty_like(q), torch.empty_like(k)]
+    buf = torch.zeros(4 * 2 * 64, device=DEV)
+    on_w, on_f, on_pos = buf[64:128], buf[300:332], buf[100:108].view(torch.int64)
+    for args in ((q, k, on_w, w[1], pos, f), (q, k, w[0], on_w, pos, f), (q, k, *w, on_pos, f), (q, k, *w, pos, on_f)):
+        for i in (0, 1):
+            out = new()
+            out[i] = buf[:out[i].numel()].view(out[i].shape) if i == 0 else buf[64:320].view(out[i].shape)
+            with pytest.raises(RuntimeError, match="overlaps"):
+                m.forward(*args, *out)
+            with pytest.raises(RuntimeError, match="overlaps"):
+                m.backward(*args, *new(), *out, None, None)
+    grads = lambda **kw: m.backward(q, k, *w, pos, f, kw.get("dqo", torch.ones_like(q)), kw.get("dko", torch.ones_like(k)),
+                                    kw.get("dq", torch.empty_like(q)), kw.get("dk", torch.empty_like(k)),
+                                    kw.get("dwq", torch.empty(64, device=DEV)), kw.get("dwk", torch.empty(64, device=DEV)))
+    a, b = new()
+    for kw in (dict(dq=a, dwq=a[1, 1]), dict(dq=a, dwk=a[3, 0]), dict(dk=b, dwq=b[2, 0]), dict(dqo=a, dwk=a[0, 0]), dict(dko=b, dwk=b[3, 0]),
+               dict(dwq=q[1, 0]), dict(dwk=q[0, 0]), dict(dwq=k[3, 0]), dict(dwq=w[1]), dict(dwk=w[0])):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            grads(**kw)
+    # in place of its own weights
+    want = [torch.empty(64, device=DEV) for _ in range(2)]
+    grads(dwq=want[0], dwk=want[1])
+    grads(dwq=w[0], dwk=w[1])
+    assert torch.equal(w[0], want[0]) and torch.equal(w[1], want[1])
+
+
 # ------------------------------------------------------------------------------------------------
 # tree attention
 # ------------------------------------------------------------------------------------------------
