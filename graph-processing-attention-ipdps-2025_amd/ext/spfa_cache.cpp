@@ -31,11 +31,11 @@ spfa_cache_t check_call(const torch::Tensor& k, const torch::Tensor& v, const to
 void spfa_cache_write_py(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor k_cache, torch::Tensor v_cache,
                          OptTensor k_scale, OptTensor v_scale) {
   const spfa_cache_t c = check_call(k, v, slots, k_cache, v_cache, k_scale, v_scale, "k and v");
-  spfa_ext::check_output(k_cache, "k_cache", {k, v, slots, v_cache});
-  spfa_ext::check_output(v_cache, "v_cache", {k, v, slots});
+  spfa_ext::check_output(k_cache, "k_cache", {k, v, slots, v_cache, k_scale, v_scale});
+  spfa_ext::check_output(v_cache, "v_cache", {k, v, slots, k_scale, v_scale});
   if (c.code != SPFA_CODE_NONE) {
-    spfa_ext::check_output(*k_scale, "k_scale", {*v_scale});
-    spfa_ext::check_output(*v_scale, "v_scale", {});
+    spfa_ext::check_output(*k_scale, "k_scale", {k, v, slots, v_scale});
+    spfa_ext::check_output(*v_scale, "v_scale", {k, v, slots});
   }
   c10::DeviceGuard guard(k.device());
   const spfa_heads_t kh = spfa_ext::heads_of(k), vh = spfa_ext::heads_of(v);
@@ -47,8 +47,8 @@ std::tuple<torch::Tensor, torch::Tensor> spfa_cache_read_py(torch::Tensor k_cach
                                                             torch::Tensor k_out, torch::Tensor v_out, OptTensor k_scale,
                                                             OptTensor v_scale) {
   const spfa_cache_t c = check_call(k_out, v_out, slots, k_cache, v_cache, k_scale, v_scale, "k_out and v_out");
-  spfa_ext::check_output(k_out, "k_out", {k_cache, v_cache, slots, v_out});
-  spfa_ext::check_output(v_out, "v_out", {k_cache, v_cache, slots});
+  spfa_ext::check_output(k_out, "k_out", {k_cache, v_cache, slots, v_out, k_scale, v_scale});
+  spfa_ext::check_output(v_out, "v_out", {k_cache, v_cache, slots, k_scale, v_scale});
   c10::DeviceGuard guard(k_out.device());
   const spfa_heads_t kh = spfa_ext::heads_of(k_out), vh = spfa_ext::heads_of(v_out);
   spfa_ext::raise_on_error(spfa_cache_read(&c, slots.data_ptr(), spfa_ext::signed_index_bytes(slots, "slots"), slots.size(0), &kh,

@@ -113,6 +113,53 @@ def test_rope_outputs_over_weights_positions_and_each_other_are_refused():
 
 
 # ------------------------------------------------------------------------------------------------
+# cache
+# ------------------------------------------------------------------------------------------------
+def test_cache_outputs_over_scales_rows_and_slots_are_refused():
+    m = _mod("spfa_cache")
+    pages, page, heads, d, n = 3, 4, 2, 64, 6
+    codes = lambda: torch.zeros(pages, page, heads, d, dtype=torch.int8, device=DEV)
+    scales = lambda: torch.zeros(pages, page, heads, device=DEV)
+    buf = torch.zeros(pages * page * heads * d, dtype=torch.int8, device=DEV)
+    over = buf.view(pages, page, heads, d)
+    on_scale = buf[512:512 + 4 * pages * page * heads].view(F32).view(pages, page, heads)
+    on_rows = buf[256:256 + n * heads * d].view(BF16).view(n, heads, d // 2)
+    on_slots = buf[128:128 + 8 * n].view(torch.int64)
+    k = torch.randn(n, heads, d, generator=_gen(1), device=DEV).to(BF16)
+    slots = torch.arange(n, device=DEV)
+    for args in ((k, k, slots, over, codes(), on_scale, scales()), (k, k, slots, over, codes(), scales(), on_scale),
+                 (k, k, slots, codes(), over, on_scale, scales()), (k, k, slots, codes(), over, scales(), on_scale),
+                 (k, k, on_slots, over, codes(), scales(), scales()), (k, k, on_slots, codes(), over, scales(), scales())):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            m.write(*args)
+    half = [torch.zeros(pages, page, heads, d // 2, dtype=torch.int8, device=DEV) for _ in range(2)]
+    rows = torch.zeros(n, heads, d // 2, dtype=BF16, device=DEV)
+    for i in (0, 1):  # a scale over rows and over slots
+        for x, s, y in ((on_rows, slots, on_scale), (rows, on_slots, buf[64:64 + 4 * pages * page * heads].view(F32).view(pages, page, heads))):
+            sc = [scales(), scales()]
+            sc[i] = y
+            with pytest.raises(RuntimeError, match="overlaps"):
+                m.write(x, rows, s, *half, *sc)
+            with pytest.raises(RuntimeError, match="overlaps"):
+                m.write(rows, x if s is slots else rows, s, *half, *sc)
+            out = [torch.zeros_like(rows), torch.zeros_like(rows)]
+            out[i] = on_rows
+            with pytest.raises(RuntimeError, match="overlaps"):
+                m.read(*half, slots, *out, on_scale, scales())
+    # codes and scales side by side in one buffer lie in each other's gaps
+    packed = torch.zeros(2, pages, page, heads, d + 8, dtype=torch.int8, device=DEV)
+    kc, vc = packed[0, ..., :d], packed[1, ..., :d]
+    ks, vs = [packed[i, ..., d:d + 4].view(F32).squeeze(-1) for i in (0, 1)]
+    m.write(k, k, slots, kc, vc, ks, vs)
+    out = [torch.empty_like(k), torch.empty_like(k)]
+    m.read(kc, vc, slots, *out, ks, vs)
+    want, amax = sv.quantise(np64(k), "int8")
+    want = want * (amax / 127)[..., None]
+    for x in out:
+        _close(x, want, (HALF[BF16] + 4 * U) * np.abs(want), "read back")
+
+
+# ------------------------------------------------------------------------------------------------
 # tree attention
 # ------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("far", [14.25, 17.46875])
