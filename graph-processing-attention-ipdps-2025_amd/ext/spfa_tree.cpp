@@ -72,8 +72,11 @@ torch::Tensor spfa_tree_forward_py(torch::Tensor q, torch::Tensor k_cache, torch
   t.l = l.has_value() ? (float*)l->data_ptr() : nullptr;
   t.scale = scale.has_value() ? (float)*scale : 1.f / std::sqrt((float)c.d);
   // (a row of q is read by every workgroup that has a part of its keys, so out cannot take its place)
-  spfa_ext::check_output(out, "out", {q, k_cache, v_cache, page_table, ctx_lens, q_offsets});
-  if (m.has_value()) spfa_ext::check_output(*m, "m", {*l});
+  spfa_ext::check_output(out, "out", {q, k_cache, v_cache, page_table, ctx_lens, q_offsets, tree_mask, k_scale, v_scale, m, l});
+  if (m.has_value()) {
+    spfa_ext::check_output(*m, "m", {q, k_cache, v_cache, page_table, ctx_lens, q_offsets, tree_mask, k_scale, v_scale, l});
+    spfa_ext::check_output(*l, "l", {q, k_cache, v_cache, page_table, ctx_lens, q_offsets, tree_mask, k_scale, v_scale});
+  }
   c10::DeviceGuard guard(q.device());
   torch::Tensor ws = spfa_ext::make_workspace(spfa_tree_workspace_bytes(&c, &t), q);
   spfa_ext::raise_on_error(spfa_tree_forward(&c, &t, ws.data_ptr(), (size_t)ws.numel(), spfa_ext::current_stream(q)));

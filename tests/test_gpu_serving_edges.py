@@ -235,3 +235,35 @@ def test_tree_infinities_in_front_of_the_tree(dt, code, d, nodes):
                 rel = eps_p + (2 * lv.shape[1] + 40) * U + 4 * (d + 8) * U * s_abs[n]
                 tol = HALF[dt] * np.abs(w[fine]) + a[n][fine] * rel * (1 + HALF[dt]) + TINY[dt]
                 assert (np.abs(g[fine] - w[fine]) <= tol).all(), (i, n, hq)
+
+
+def test_tree_outputs_over_what_the_call_reads_are_refused():
+    r = Run(47, BF16, "int8", 64, 16, 2, 2, True, [20], [3], "tree", strided=False)
+    kc, vc, ks, vs = r.cache
+    rows = 3
+    buf = torch.zeros(1 << 16, dtype=torch.uint8, device=DEV)
+    over = lambda like, dt=None: buf[:like.numel() * like.element_size()].view(dt or like.dtype).view(like.shape)
+    new = lambda: torch.empty(r.q.shape, dtype=BF16, device=DEV)
+    state = lambda: [torch.full((rows, 4), float("-inf"), device=DEV), torch.zeros(rows, 4, device=DEV)]
+    m = _mod("spfa_tree")
+    names = ["q", "k_cache", "v_cache", "page_table", "ctx_lens", "q_offsets", "out", "tree_mask", "k_scale", "v_scale"]
+    args = lambda **kw: {**dict(zip(names, (r.q, kc.contiguous(), vc.contiguous(), r.table, r.ctx_t, r.off_t, new(), r.mask, ks.contiguous(), vs.contiguous()))), **kw}
+    m.forward(**args())
+    base = args()
+    for name in names:
+        if name == "out":
+            continue
+        at = over(base[name])
+        at.copy_(base[name])
+        with pytest.raises(RuntimeError, match="out overlaps"):
+            m.forward(**args(**{name: at, "out": over(new(), BF16)}))
+        for i, what in enumerate("ml"):
+            ml = state()
+            ml[i] = buf[:48].view(F32).view(rows, 4)
+            with pytest.raises(RuntimeError, match="%s overlaps" % what):
+                m.forward(**args(**{name: at}), m=ml[0], l=ml[1])
+    for i in (0, 1):
+        ml = state()
+        ml[i] = buf[16:64].view(F32).view(rows, 4)
+        with pytest.raises(RuntimeError, match="out overlaps"):
+            m.forward(**args(out=over(new(), BF16)), m=ml[0], l=ml[1])
