@@ -70,10 +70,11 @@ TreePlan tree_plan(const spfa_cache_t* c, const spfa_tree_t* t) {
   if (keys > (double)c->pages * (double)c->page_size) keys = (double)c->pages * (double)c->page_size;
   // The wide kernel takes a key's way through LDS once for 128 rows, but has to fill, store and join 128:
   // it gains once they are more than two of the narrow kernel's tiles and its workgroups have many blocks.
-  // Us, narrow against wide, 8 sequences and 4 heads: 64 bf16/f16 elements, 96 rows of 2900 keys 28 / 35, of
-  // 20000 84 / 66, 512 of 8000 110 / 86; 128 bf16 elements, 128 rows of 20000 192 / 183, 512 of 8000
-  // 232 / 216, of 2900 97 / 106; 128 int8 elements, 128 rows of 20000 127 / 127, 192 179 / 203, 512 of 40000
-  // 770 / 651; 256 elements, 128 rows of 20000 bf16 495 / 400, e4m3 313 / 344, 512 of 8000 466 / 452.
+  // Us, narrow against wide, 8 sequences and 4 heads: 64 elements, 96 rows of 2900 keys f16 26 / 34, bf16 27 / 37,
+  // of 20000 85 / 63 and 86 / 74, 512 of 8000 98 / 81 and 103 / 94; 128 bf16 elements, 192 rows of 8000
+  // 108 / 117, of 20000 288 / 242, 512 of 20000 660 / 421 (the limit leaves some: 128 of 20000 187 / 164, 512 of 8000
+  // 224 / 185); 128 int8 elements, 128 rows of 20000 120 / 121, 192 164 / 180, 256 206 / 183, 512 379 / 323;
+  // 256 elements, 128 rows of 20000 bf16 483 / 421, 256 e4m3 598 / 607, 512 1188 / 1107.
   const double per_group = (double)c->heads * (double)((rows + 127) / 128) * keys / kTreeBlock / (256 * wide_groups(s.dp));
   const bool many = rows > (c->code == SPFA_CODE_NONE || s.dp == 64 ? 64 : 192);
   s.wide = s.rows_how != kTreeAny && many && per_group >= (s.dp == 64 ? 4.0 : 16.0);

@@ -262,11 +262,9 @@ struct TreeTypes {
   static constexpr int QF = DP / 32;           // pieces of a query
   using Tv = std::conditional_t<kCoded, bf16, T>;  // (8-bit values times any scale need bf16's range)
   // Weights in two bf16 parts: needed where f16 calls meet 8-bit codes (one part has 8 of their 11 bits),
-  // and with bf16 calls what keeps the result to its own rounding (one part adds as much again).  The
-  // narrow kernel has room and time for it (2 x 200001 bf16 tokens 225 -> 226 us, 64 x 8191 e4m3 131 -> 132);
-  // the wide one's registers spill with bf16 heads of 128.
-  static constexpr bool kTwoNarrow = kCoded || __is_same(T, bf16);
-  static constexpr bool kTwoWide = kCoded && __is_same(T, f16);
+  // and with bf16 calls what keeps the result to its own rounding (one part adds as much again, and the
+  // kernels, chosen by a table's width, would differ by it).
+  static constexpr bool kTwo = kCoded || __is_same(T, bf16);
 };
 
 // This workgroup's run of the line of all items' blocks, item by item.
@@ -883,7 +881,7 @@ __global__ __launch_bounds__(256, narrow_waves(CODE, DP, NR)) void tree_narrow_k
     int t = it.blk0 * 4 + wave;
     TreeKeys<T, CODE, DP, ROWS> keys;
     TreeQueries<T, CODE, DP, ROWS> q[NR];
-    TreeState<T, CODE, DP, Ty::kTwoNarrow> st[NR];
+    TreeState<T, CODE, DP, Ty::kTwo> st[NR];
     keys.start(a, it, t_end, reinterpret_cast<int64_t*>(mine));
 #pragma unroll
     for (int n = 0; n < NR; n++) st[n].start();
@@ -1012,7 +1010,7 @@ __global__ __launch_bounds__(256, wide_groups(DP)) void tree_wide_kernel(TreeArg
     int t = it.blk0 * 4;  // first tile of the block
     TreeKeys<T, CODE, DP, ROWS> keys;
     TreeQueries<T, CODE, DP, ROWS> q[NR];
-    TreeState<T, CODE, DP, Ty::kTwoWide> st[NR];
+    TreeState<T, CODE, DP, Ty::kTwo> st[NR];
     keys.start(a, it, t_end, reinterpret_cast<int64_t*>(mine));
 #pragma unroll
     for (int n = 0; n < NR; n++) st[n].start();

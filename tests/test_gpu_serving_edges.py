@@ -267,3 +267,57 @@ def test_tree_outputs_over_what_the_call_reads_are_refused():
         ml[i] = buf[16:64].view(F32).view(rows, 4)
         with pytest.raises(RuntimeError, match="out overlaps"):
             m.forward(**args(out=over(new(), BF16)), m=ml[0], l=ml[1])
+
+
+@pytest.mark.parametrize("nodes", [5, 130])
+@pytest.mark.parametrize("code", ["none", "int8", "e4m3"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_tree_weights_of_bf16_calls_have_two_parts(d, code, nodes):
+    """Two keys whose values nearly cancel in some elements of each row: what is left of them shows the
+    weights' rounding, which is to 16 bits in the tiles of few rows and of many."""
+    r = Run(44, BF16, code, d, 16, 1, 2, True, [2], [nodes], "random", strided=False, **(dict(spare=50000, wide=50000) if nodes > 100 else {}))
+    r.mask.zero_()
+    kc, vc, ks, vs = r.cache
+    gaps = torch.tensor([0.21, 0.37, 0.58, 0.81, 1.17, 1.51, 1.93, 2.6], device=DEV)
+    r.q = torch.zeros(nodes, 2, d, dtype=BF16, device=DEV)
+    r.q[:, 0, 0] = (gaps * math.sqrt(d)).to(BF16)[torch.arange(nodes, device=DEV) % 8]
+    r.q[:, 1, 0] = (gaps * math.sqrt(d)).to(BF16)[(torch.arange(nodes, device=DEV) + 3) % 8]
+    k, v = torch.zeros(2, 1, d, device=DEV), torch.zeros(2, 1, d, device=DEV)
+    k[1, 0, 0] = -1
+    v[1] = 1 + torch.rand(1, d, generator=_gen(45), device=DEV)
+    write = lambda: _mod("spfa_cache").write(k.to(BF16), v.to(BF16), r.slots[0][:2], kc, vc, ks, vs)
+    write()
+    p = torch.exp(-(gaps * math.sqrt(d)).to(BF16).double() / math.sqrt(d))[torch.arange(d, device=DEV) % 8]
+    v[0, 0] = -(p * torch.from_numpy(r.read(0)[1][1, 0]).to(DEV)).float()  # takes the second key's back where e % 8 is the row's gap
+    write()
+    out = torch.empty(r.q.shape, dtype=BF16, device=DEV)
+    r.call(out)
+    kk, vv = r.read(0)
+    for h in (0, 1):
+        o, _, _, a, s_abs = sv.tree_attention(np64(r.q)[:, h], kk[:2, 0], vv[:2, 0], np.ones((nodes, 2), dtype=bool), 1 / math.sqrt(d))
+        rel = 2.0 ** -16 + (2 * 2 + 40) * U + 4 * (d + 8) * U * s_abs
+        _close(out[:, h], o, HALF[BF16] * np.abs(o) + a * rel[:, None] * (1 + HALF[BF16]) + TINY[BF16], "head %d" % h)
+
+
+@pytest.mark.parametrize("code", ["none", "e4m3"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_tree_tight_and_roomy_tables(d, code):
+    """The table's width and the cache's size choose the kernel, and with it the order of the sums: the same
+    rows, keys and lengths stay within their bounds of the exact result and of each other."""
+    args = (46, BF16, code, d, 16, 1, 4, True, [500, 90], [60, 50], "chain")
+    tight = Run(*args)
+    roomy = Run(*args, **ROOM)
+    assert torch.equal(tight.q, roomy.q)
+    outs = []
+    for r in (tight, roomy):
+        out = torch.empty(r.q.shape, dtype=BF16, device=DEV)
+        r.call(out)
+        r.check(out)
+        outs.append(np64(out))
+    # of each: half a step of itself, and of sum p |v| / l, at most the largest |v|, the weights' 2^-16 and
+    # what Run.check allows for sums and scores (of 560 keys)
+    v = max(np.abs(tight.read(i)[1]).max() for i in range(2))
+    q = np.abs(np64(tight.q)).sum(-1).max() * max(np.abs(tight.read(i)[0]).max() for i in range(2)) / math.sqrt(d)
+    rel = 2.0 ** -16 + (2 * 560 + 40) * U + 4 * (d + 8) * U * q
+    bound = HALF[BF16] * (np.abs(outs[0]) + np.abs(outs[1])) * 1.01 + 2 * v * rel
+    assert (np.abs(outs[0] - outs[1]) <= bound).all()
