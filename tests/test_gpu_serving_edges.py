@@ -112,6 +112,29 @@ def test_rope_outputs_over_weights_positions_and_each_other_are_refused():
     assert torch.equal(w[0], want[0]) and torch.equal(w[1], want[1])
 
 
+def test_rope_angles_next_to_quarter_turns():
+    """The sine or cosine of an angle next to a quarter of a turn is as small as what the angle lacks of it: only an
+    angle of more than 24 bits gives its leading digits."""
+    d, eps = 64, 1e-6
+    f = 500000.0 ** (-np.arange(32, dtype=np.float64) / 32)
+    f = f.astype(np.float32)
+    pos = np.arange(1 << 20, dtype=np.int64)
+    rows = []  # per frequency the positions whose angle is nearest to a whole number of quarter turns
+    for x in f[:8]:
+        t = pos[1:] * (float(x) / (math.pi / 2))
+        rows += list(pos[1:][np.argsort(np.abs(t - np.rint(t)))[:8]])
+    p = np.array(rows)
+    x = torch.zeros(len(p), 1, d, device=DEV)
+    x[..., :32] = 1  # pairs (1, 0): they become (cos, sin) of the norm
+    out = torch.empty_like(x)
+    _mod("spfa_rope").forward(x, x[:, :0], None, None, torch.from_numpy(p).to(DEV), torch.from_numpy(f).to(DEV), out, x[:, :0].clone(), eps)
+    want = sv.norm_rope(np64(x), np.ones(d), p.tolist(), f.astype(np.float64), eps, False)
+    # angles: two roundings of the product in 64 bits, here and in the oracle (half a step of the position's
+    # angle each); sine, cosine, norm and product: 20 roundings of fp32
+    angle = np.concatenate([np.abs(p[:, None] * f[None].astype(np.float64))] * 2, 1)[:, None]
+    _close(out, want, 20 * U * np.abs(want) + 4 * 2.0 ** -52 * angle * math.sqrt(2) + 2.0 ** -48, "next to a quarter")
+
+
 # ------------------------------------------------------------------------------------------------
 # cache
 # ------------------------------------------------------------------------------------------------
