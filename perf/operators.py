@@ -8,6 +8,7 @@ tree   attention of a tree of drafted tokens (or of a chain: plain decoding) ove
 Where `own` is false, run() computes a case in elementary torch operations; where it is true it makes
 the calls a user makes of this repository's modules.
 """
+import functools
 import math
 import os
 import sys
@@ -22,6 +23,7 @@ TOP = {"int8": 127.0, "e4m3": 448.0}
 EPS = 1e-6
 
 
+@functools.lru_cache(maxsize=None)  # (a user's program imports a module once, not with each call)
 def _mod(name):
     import importlib
     here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
