@@ -11,8 +11,8 @@
 // once in fp64 (position * frequency / 2 pi, less its nearest whole number), takes sine and cosine of
 // its fp32 form, adds what that form left of the angle, and keeps them in LDS for the vectors of its tokens.
 //
-// Measured, 16384 tokens of 32 + 8 bf16 heads of 128: forward 69 us (4.9 TB/s, what a copy reaches),
-// gradients 128 us (3.9 TB/s; 193 registers leave two wavefronts per SIMD, fewer registers by one vector
+// Measured, 16384 tokens of 32 + 8 bf16 heads of 128: forward 68 us (4.9 TB/s, what a copy reaches),
+// gradients 124 us (4.0 TB/s; 191 registers leave two wavefronts per SIMD, fewer registers by one vector
 // on the way instead of two: 137 us, by spilling: 171) and 5 us for the weights' sum; one token 4 us.
 #include <type_traits>
 

@@ -262,8 +262,10 @@ struct TreeTypes {
   static constexpr int QF = DP / 32;           // pieces of a query
   using Tv = std::conditional_t<kCoded, bf16, T>;  // (8-bit values times any scale need bf16's range)
   // Weights in two bf16 parts: needed where f16 calls meet 8-bit codes (one part has 8 of their 11 bits),
-  // and with bf16 calls what keeps the result to its own rounding (one part adds as much again, and the
-  // kernels, chosen by a table's width, would differ by it).
+  // and with bf16 calls what keeps the result to its own rounding (error against 64 bits 0.0017, with one part
+  // 0.0023; in the kernel of many rows 124 -> 149 us for 64 elements, 333 -> 288 for 128, 8 x 20000 tokens, 512 rows
+  // for each of 4 heads).  f16 calls over f16 have one part, of the result's own 11 bits, in both kernels: 0.00027
+  // with many rows where two parts have 0.00021 (f16's rounding), for 76 us instead of 64 at 488 rows of 5000 keys.
   static constexpr bool kTwo = kCoded || __is_same(T, bf16);
 };
 
@@ -839,9 +841,11 @@ __device__ __forceinline__ void wait_loads() {
 
 // 16 NR rows per item (plain decoding, small trees): the wavefronts deal an item's keys among themselves,
 // tile by tile, and run apart until its end.  Bound by the reads of K and V where the rows are few: 64 e4m3
-// sequences of up to 8191 tokens, 8 heads of 128, 131 us (5.3 TB/s of the 6.0 to 6.4 that plain reads reach);
-// 2 of up to 200001 bf16 tokens 224 us (5.6 TB/s).  With 70 to 90 rows over int8 (16 sequences of up to 12345)
-// the softmax and the decoding of codes bound it, 80 us; 32-row tiles there instead of 16 halve the decoding.
+// sequences of up to 8191 tokens, 8 heads of 128, 133 us (5.2 TB/s of the 6.0 to 6.4 that plain reads reach);
+// 2 of up to 200001 bf16 tokens 225 us (5.6 TB/s).  With 70 to 90 rows over int8 (16 sequences of up to 12345)
+// the softmax and the decoding of codes bound it, 82 us; 32-row tiles there instead of 16 halve the decoding.
+// Registers end at two wavefronts per SIMD: 32-row tiles of 128 plain elements spill 17 to 20 of them, 8-bit ones
+// of 256 2 to 30.
 template <int DP, int NR>
 struct NarrowLds {
   static constexpr int kRows = 16 * NR * kTreeWaves, kStride = DP + 4;
@@ -970,7 +974,9 @@ __global__ __launch_bounds__(256, narrow_waves(CODE, DP, NR)) void tree_narrow_k
 // into LDS in the form the products take them (so looking up, decoding and reordering is done once for
 // all rows), then works on its own 32 rows.  One buffer: while a workgroup refills it, the CU's other one
 // computes.  Bound by the softmax's vector instructions (exponentials, packing, maxima): 6 sequences of up
-// to 5000 tokens, 488 rows for each of 8 heads of 64, 55 us and the merge 9 us; over long contexts 430 TFLOP/s.
+// to 5000 tokens, 488 rows for each of 8 f16 heads of 64, 56 us and the merge 9 us; 8 of up to 20000, 512 rows for
+// each of 4, 114 us (430 TFLOP/s), bf16 138, bf16 heads of 128 288 us (340 TFLOP/s).  Heads of 64 have registers
+// enough; with 128 elements 56 to 157 of them spill, with 256 170 to 584, which those sizes pay for.
 template <int DP>
 struct WideLds {
   static constexpr int kRows = 32 * kTreeWaves;
